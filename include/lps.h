@@ -57,6 +57,8 @@ enum {
 
 /* Logits element types. */
 enum { LPS_DTYPE_F32 = 0, LPS_DTYPE_BF16 = 1, LPS_DTYPE_F16 = 2 };
+/* Microscaled 4-bit floats (lps_mx4_quantize), where a call says it takes them. */
+enum { LPS_DTYPE_MX4 = 3 };
 
 /* Per-row status bits written to row_status[] by the kernels.  A set bit on a
  * sampling row corresponds to the RuntimeError torch.multinomial raises for an
@@ -351,6 +353,115 @@ int lps_lm_head(const lps_lm_head_args* args, void* stream);
 size_t lps_softmax_workspace_bytes(int rows, int cols, int dtype);
 
 int lps_softmax(const lps_softmax_args* args, void* stream);
+
+/* ------------------------------------------------------------------------
+ * The vocabulary table: one [vocab, hidden] table at both ends of a decode
+ * loop (the sampled token's row in, the LM head's products out), in 16 or 32
+ * bits or as microscaled 4-bit floats.
+ *
+ * 4-bit form of a row: blocks of 32 values (the last may hold fewer), 16 bytes
+ * of codes and one scale byte a block.  Scale byte b stands for 2^(b - 127),
+ * 255 for NaN.  A code is a sign (8) and the index of one of 0, 0.5, 1, 1.5, 2,
+ * 3, 4, 6; element 2 j of a block is the low half of its byte j.
+ * -------------------------------------------------------------------- */
+#define LPS_MX4_BLOCK 32
+
+/* lps_mx4_quantize: x to codes and scales.  A block's scale is 2^s, s =
+ * max(floor(log2(largest magnitude)) - 2, -126), its codes the nearest values
+ * to x / 2^s (ties to the even code, 6 above it, the sign kept for zeros); a
+ * block with a value that is not finite becomes scale 255, codes 0.  Values
+ * past a row's end count as zeros.
+ * lps_mx4_dequantize: codes and scales to x (rounded to x's type).
+ * Code rows begin on 4-byte lines; everything else at any element. */
+typedef struct lps_mx4_args {
+  void* x;                        /* [rows, hidden] in dtype */
+  void* codes;                    /* uint8 [rows, 16 * ceil(hidden / 32)] */
+  void* scales;                   /* uint8 [rows, ceil(hidden / 32)] */
+  int32_t dtype;                  /* lps_dtype of x: F32, BF16 or F16 */
+  int32_t rows;
+  int32_t hidden;
+  int64_t x_stride;               /* elements */
+  int64_t codes_stride;           /* bytes, a multiple of 4 */
+  int64_t scales_stride;          /* bytes */
+} lps_mx4_args;
+
+int lps_mx4_quantize(const lps_mx4_args* args, void* stream);
+int lps_mx4_dequantize(const lps_mx4_args* args, void* stream);
+
+/* LM head over a 4-bit weight, lps_lm_head otherwise (logits, statistics):
+ * x in bf16, fp16 or 4 bits.  Any hidden; the codes of w past a row's end count
+ * as zeros, those of a 4-bit x must be (lps_mx4_quantize leaves them so).
+ * Rows of x and w begin on 16-byte lines, rows of scales on 4-byte lines. */
+typedef struct lps_lm_head_mx4_args {
+  const void* x;                  /* [rows, hidden] in dtype; 4-bit codes */
+  const void* x_scales;           /* 4-bit x: uint8 [rows, ceil(hidden / 32)] */
+  const void* w;                  /* codes, uint8 [vocab, 16 * ceil(hidden / 32)] */
+  const void* w_scales;           /* uint8 [vocab, ceil(hidden / 32)] */
+  void* out;                      /* [rows, vocab] in out_dtype */
+  float* stats;                   /* float32 [rows, ceil(vocab / 128), 2] or NULL */
+  int32_t dtype;                  /* of x: BF16, F16 or MX4 */
+  int32_t out_dtype;              /* F32, BF16 or F16 */
+  int32_t rows;
+  int32_t vocab;
+  int32_t hidden;
+  int64_t x_stride;               /* elements, a multiple of 8; bytes of 4-bit codes, of 16 */
+  int64_t x_scales_stride;        /* bytes, a multiple of 4 */
+  int64_t w_stride;               /* bytes, a multiple of 16 */
+  int64_t w_scales_stride;        /* bytes, a multiple of 4 */
+  int64_t out_stride;             /* elements */
+} lps_lm_head_mx4_args;
+
+int lps_lm_head_mx4(const lps_lm_head_mx4_args* args, void* stream);
+
+/* Embedding lookup: out[i] = scale * table[ids[i]] (fp32 arithmetic, rounded
+ * once to out_dtype), zeros for ids outside [0, vocab) (-1 is what sampling and
+ * verification leave where there is no token). */
+typedef struct lps_embedding_args {
+  const void* ids;                /* [n] */
+  const void* table;              /* [vocab, hidden] in dtype; 4-bit codes */
+  const void* scales;             /* 4-bit tables: uint8 [vocab, ceil(hidden / 32)] */
+  void* out;                      /* [n, hidden] in out_dtype */
+  int32_t id_bytes;               /* 8 or 4: int64 or int32 ids */
+  int32_t dtype;                  /* lps_dtype of the table: F32, BF16, F16 or MX4 */
+  int32_t out_dtype;              /* F32, BF16 or F16 */
+  int32_t n;
+  int32_t vocab;
+  int32_t hidden;
+  int64_t table_stride;           /* elements; bytes of 4-bit codes (a multiple of 4) */
+  int64_t scales_stride;          /* bytes */
+  int64_t out_stride;             /* elements */
+  float scale;
+} lps_embedding_args;
+
+int lps_embedding(const lps_embedding_args* args, void* stream);
+
+/* Gradient of the lookup in its table:
+ *   out[v] = scale * sum of grad[i] over the i with ids[i] = v
+ * (ids outside [0, vocab) add nothing), on top of out[v] with accumulate (rows
+ * without an id are then not touched).  Summed in fp32, rounded once, in an
+ * order that depends on ids and sizes alone: equal calls give equal bits.
+ * workspace: lps_embedding_grad_workspace_bytes(n, vocab, hidden) bytes, 16-byte
+ * aligned, of any content; calls that overlap in time must not share it. */
+typedef struct lps_embedding_grad_args {
+  const void* ids;                /* [n] */
+  const void* grad;               /* [n, hidden] in dtype */
+  void* out;                      /* [vocab, hidden] in out_dtype */
+  int32_t id_bytes;               /* 8 or 4 */
+  int32_t dtype;                  /* F32, BF16 or F16 */
+  int32_t out_dtype;              /* F32, BF16 or F16 */
+  int32_t n;
+  int32_t vocab;
+  int32_t hidden;
+  int64_t grad_stride;            /* elements */
+  int64_t out_stride;             /* elements */
+  float scale;
+  int32_t accumulate;             /* 0 / 1 */
+  void* workspace;
+  size_t workspace_bytes;
+} lps_embedding_grad_args;
+
+size_t lps_embedding_grad_workspace_bytes(int n, int vocab, int hidden);
+int lps_embedding_grad(const lps_embedding_grad_args* args, void* stream);
 
 #ifdef __cplusplus
 }

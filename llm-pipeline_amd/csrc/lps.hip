@@ -1,13 +1,13 @@
 // C ABI of the lps token sampler (declarations and reference citations are in
 // include/lps.h).  Launches only; no allocation, no synchronisation.  The only
 // process-wide state is per-device and write-once: the CU count of each device
-// (atomic entries) and the no-allocation entry point's workspace address
+// (atomic entries, lps_host.h) and the no-allocation entry point's workspace address
 // (std::call_once per device).
 #include <hip/hip_runtime.h>
 
-#include <atomic>
 #include <mutex>
 
+#include "lps_host.h"
 #include "lps_rowgroup.h"
 #include "lps_stream.h"
 #include "lps_generic.h"
@@ -46,8 +46,6 @@ bool vec_ok(const void* base, int dtype, int V, int rows_inner, int64_t so, int6
   return true;
 }
 
-bool dtype_ok(int d) { return d == LPS_DTYPE_F32 || d == LPS_DTYPE_BF16 || d == LPS_DTYPE_F16; }
-
 size_t round_up(size_t x, size_t m) { return (x + m - 1) / m * m; }
 
 // Row-group workspace: per-row counters (a fixed region at offset 0, so a
@@ -67,22 +65,6 @@ struct RgWs {
 
 // Rows per row-group launch; larger batches are split into launches.
 constexpr int RG_MAX_ROWS = 1024;
-
-// CUs of the current device (cached per device): one resident round of
-// row-group workgroups.
-// (threads that race on a device's first call each store the same value)
-std::atomic<int> g_cus[64];
-int device_cus() {
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
-  int c = g_cus[dev].load(std::memory_order_relaxed);
-  if (!c) {
-    int n = 0;
-    c = (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && n > 0) ? n : 256;
-    g_cus[dev].store(c, std::memory_order_relaxed);
-  }
-  return c;
-}
 
 // Whether a launch needs the row-group kernel's build with the extra features:
 // the entropy output, the mass-only path for pure rows without a draw (top_p

@@ -1,0 +1,85 @@
+// C ABI of the LM head over a 4-bit weight (declaration in include/lps.h).
+// Launches only; no allocation, no synchronisation.
+#include <hip/hip_runtime.h>
+
+#include "lps_host.h"
+#include "lps_mx4head.h"
+
+using namespace lps;
+
+namespace {
+
+template <int XDT, int ODT, typename T, bool NTL>
+hipError_t launch_mx4head(Mx4HeadParams Q, hipStream_t s) {
+  Q.h.mtiles = (Q.h.M + T::BM - 1) / T::BM;
+  Q.h.tiles = Q.h.mtiles * ((Q.h.V + T::BN - 1) / T::BN);
+  hipLaunchKernelGGL((mx4head_kernel<XDT, ODT, T, NTL>), dim3((unsigned)(Q.h.tiles + 7) / 8 * 8), dim3(T::NT), 0, s, Q);
+  return hipGetLastError();
+}
+int mx4head_shape(int M) { return M <= 32 ? 0 : M <= 64 ? 1 : M <= 128 ? 2 : 3; }
+
+template <int XDT, int ODT>
+hipError_t launch_mx4head_rows(const Mx4HeadParams& Q, hipStream_t s) {
+  constexpr int XB = XDT == DT_MX4 ? 16 : 64;
+  switch (mx4head_shape(Q.h.M)) {
+    case 0: return launch_mx4head<XDT, ODT, M4Tile<32, 128, 1, 4, 6, 1, XB>, true>(Q, s);
+    case 1: return launch_mx4head<XDT, ODT, M4Tile<64, 128, 1, 4, 5, 1, XB>, true>(Q, s);
+    case 2: return launch_mx4head<XDT, ODT, M4Tile<128, 128, 4, 2, 3, 2, XB>, true>(Q, s);
+    default:
+      if constexpr (XB == 16) return launch_mx4head<XDT, ODT, M4Tile<256, 256, 4, 2, 4, 2, XB>, false>(Q, s);
+      else return launch_mx4head<XDT, ODT, M4Tile<128, 256, 2, 4, 3, 2, XB>, false>(Q, s);
+  }
+}
+template <int XDT>
+hipError_t dispatch_mx4head(const Mx4HeadParams& Q, int out_dtype, hipStream_t s) {
+  switch (out_dtype) {
+    case LPS_DTYPE_F32: return launch_mx4head_rows<XDT, LPS_DTYPE_F32>(Q, s);
+    case LPS_DTYPE_BF16: return launch_mx4head_rows<XDT, LPS_DTYPE_BF16>(Q, s);
+    default: return launch_mx4head_rows<XDT, LPS_DTYPE_F16>(Q, s);
+  }
+}
+
+}  // namespace
+
+extern "C" int lps_lm_head_mx4(const lps_lm_head_mx4_args* a, void* stream) {
+  if (!a) return LPS_EINVAL;
+  const bool x4 = a->dtype == LPS_DTYPE_MX4;
+  if (!x4 && a->dtype != LPS_DTYPE_BF16 && a->dtype != LPS_DTYPE_F16) return LPS_EUNSUPPORTED_DTYPE;
+  if (!dtype_ok(a->out_dtype)) return LPS_EUNSUPPORTED_DTYPE;
+  if (a->rows < 0 || a->vocab < 1 || a->hidden < 1 || a->rows > LMH_MAX_ROWS) return LPS_EINVAL;
+  if (a->rows == 0) return LPS_OK;
+  if (!a->x || !a->w || !a->w_scales || !a->out || (x4 && !a->x_scales)) return LPS_EINVAL;
+  const int64_t nb = ((int64_t)a->hidden + MX4_BLOCK - 1) / MX4_BLOCK;
+  Mx4HeadParams Q{};
+  LmHeadParams& P = Q.h;
+  // (a single row's stride does not count)
+  P.x_stride = a->rows > 1 ? a->x_stride : 0;
+  P.w_stride = a->vocab > 1 ? a->w_stride : 0;
+  P.out_stride = a->rows > 1 ? a->out_stride : a->vocab;
+  Q.ws_stride = a->vocab > 1 ? a->w_scales_stride : 0;
+  Q.xs_stride = x4 && a->rows > 1 ? a->x_scales_stride : 0;
+  if (a->rows > 1 && (P.x_stride < (x4 ? 16 * nb : a->hidden) || P.out_stride < a->vocab)) return LPS_EINVAL;
+  if (a->vocab > 1 && (P.w_stride < 16 * nb || Q.ws_stride < nb)) return LPS_EINVAL;
+  if (x4 && a->rows > 1 && Q.xs_stride < nb) return LPS_EINVAL;
+  // 16-byte operand loads, 4-byte loads of scales
+  if (reinterpret_cast<uintptr_t>(a->x) % 16 || P.x_stride % (x4 ? 16 : 8) || reinterpret_cast<uintptr_t>(a->w) % 16 ||
+      P.w_stride % 16)
+    return LPS_EINVAL;
+  if (reinterpret_cast<uintptr_t>(a->w_scales) % 4 || Q.ws_stride % 4) return LPS_EINVAL;
+  if (x4 && (reinterpret_cast<uintptr_t>(a->x_scales) % 4 || Q.xs_stride % 4)) return LPS_EINVAL;
+  P.x = a->x;
+  P.w = a->w;
+  P.out = a->out;
+  P.stats = a->stats;
+  P.M = a->rows;
+  P.V = a->vocab;
+  P.H = a->hidden;
+  P.G = (a->vocab + LMH_BN - 1) / LMH_BN;
+  Q.ws = static_cast<const uint8_t*>(a->w_scales);
+  Q.xs = static_cast<const uint8_t*>(a->x_scales);
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const hipError_t e = x4 ? dispatch_mx4head<DT_MX4>(Q, a->out_dtype, s)
+                       : a->dtype == LPS_DTYPE_BF16 ? dispatch_mx4head<LPS_DTYPE_BF16>(Q, a->out_dtype, s)
+                                                    : dispatch_mx4head<LPS_DTYPE_F16>(Q, a->out_dtype, s);
+  return e == hipSuccess ? LPS_OK : LPS_ELAUNCH;
+}

@@ -12,6 +12,7 @@ from .softmax import fused_softmax, fused_softmax_triton
 from .spec_driver import (mtp_speculative_decode, mtp_speculative_decode_batched, speculative_decode,
                           speculative_decode_batched)
 from .state import SamplerState
+from .vocab_table import Mx4Tensor, embedding, embedding_grad, mx4_dequantize, mx4_quantize
 
 __all__ = [
     "Sampler",
@@ -30,6 +31,11 @@ __all__ = [
     "verify_drafts_batched",
     "spec_verify",
     "lm_head",
+    "Mx4Tensor",
+    "mx4_quantize",
+    "mx4_dequantize",
+    "embedding",
+    "embedding_grad",
     "speculative_decode",
     "speculative_decode_batched",
     "mtp_speculative_decode",

@@ -26,6 +26,9 @@ LPS_NOALLOC_WORKSPACE_BYTES = 16 << 20
 LPS_DTYPE_F32 = 0
 LPS_DTYPE_BF16 = 1
 LPS_DTYPE_F16 = 2
+LPS_DTYPE_MX4 = 3   # microscaled 4-bit floats, where a call takes them
+
+LPS_MX4_BLOCK = 32
 
 LPS_ROW_NONFINITE = 1
 LPS_ROW_EMPTY = 2
@@ -108,6 +111,46 @@ class SpecArgs(ctypes.Structure):
     ]
 
 
+class Mx4Args(ctypes.Structure):
+    """Mirror of ``lps_mx4_args``."""
+
+    _fields_ = [
+        ("x", _vp), ("codes", _vp), ("scales", _vp), ("dtype", _i32), ("rows", _i32), ("hidden", _i32),
+        ("x_stride", _i64), ("codes_stride", _i64), ("scales_stride", _i64),
+    ]
+
+
+class LmHeadMx4Args(ctypes.Structure):
+    """Mirror of ``lps_lm_head_mx4_args``."""
+
+    _fields_ = [
+        ("x", _vp), ("x_scales", _vp), ("w", _vp), ("w_scales", _vp), ("out", _vp), ("stats", _vp),
+        ("dtype", _i32), ("out_dtype", _i32), ("rows", _i32), ("vocab", _i32), ("hidden", _i32),
+        ("x_stride", _i64), ("x_scales_stride", _i64), ("w_stride", _i64), ("w_scales_stride", _i64),
+        ("out_stride", _i64),
+    ]
+
+
+class EmbeddingArgs(ctypes.Structure):
+    """Mirror of ``lps_embedding_args``."""
+
+    _fields_ = [
+        ("ids", _vp), ("table", _vp), ("scales", _vp), ("out", _vp), ("id_bytes", _i32), ("dtype", _i32),
+        ("out_dtype", _i32), ("n", _i32), ("vocab", _i32), ("hidden", _i32), ("table_stride", _i64),
+        ("scales_stride", _i64), ("out_stride", _i64), ("scale", _f32),
+    ]
+
+
+class EmbeddingGradArgs(ctypes.Structure):
+    """Mirror of ``lps_embedding_grad_args``."""
+
+    _fields_ = [
+        ("ids", _vp), ("grad", _vp), ("out", _vp), ("id_bytes", _i32), ("dtype", _i32), ("out_dtype", _i32),
+        ("n", _i32), ("vocab", _i32), ("hidden", _i32), ("grad_stride", _i64), ("out_stride", _i64),
+        ("scale", _f32), ("accumulate", _i32), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 # Every symbol include/lps.h declares, with its ctypes signature.
 SIGNATURES = {
     "lps_version": (_i32, []),
@@ -121,6 +164,12 @@ SIGNATURES = {
     "lps_softmax": (_i32, [ctypes.c_void_p, _vp]),
     "lps_softmax_workspace_bytes": (ctypes.c_size_t, [_i32, _i32, _i32]),
     "lps_lm_head": (_i32, [ctypes.c_void_p, _vp]),
+    "lps_mx4_quantize": (_i32, [ctypes.c_void_p, _vp]),
+    "lps_mx4_dequantize": (_i32, [ctypes.c_void_p, _vp]),
+    "lps_lm_head_mx4": (_i32, [ctypes.c_void_p, _vp]),
+    "lps_embedding": (_i32, [ctypes.c_void_p, _vp]),
+    "lps_embedding_grad_workspace_bytes": (ctypes.c_size_t, [_i32, _i32, _i32]),
+    "lps_embedding_grad": (_i32, [ctypes.c_void_p, _vp]),
     "lps_selftest_exp2_monotone": (_i32, [ctypes.POINTER(ctypes.c_ulonglong)]),
 }
 

@@ -1,4 +1,5 @@
-"""In-tree build of ``liblps.so`` for gfx950 with hipcc.
+"""In-tree build of ``liblps.so`` for gfx950 with hipcc: the translation units
+of ``csrc/`` side by side, then one link.
 
 Flags: ``-ffp-contract=off`` and correctly rounded fp32 division keep the
 penalty / temperature arithmetic bit-identical to IEEE fp32; packed-fp32 ops
@@ -8,6 +9,7 @@ from __future__ import annotations
 
 import os
 import subprocess
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG_ROOT = os.path.dirname(HERE)                    # llm-pipeline_amd/
@@ -18,7 +20,7 @@ OUT = os.path.join(HERE, "liblps.so")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [
-    "--offload-arch=gfx950", "-O3", "-std=c++17", "-shared", "-fPIC",
+    "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
     "-ffp-contract=off", "-fhip-fp32-correctly-rounded-divide-sqrt",
     "-Wall", "-Werror=return-type", "-Werror=uninitialized",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
@@ -28,17 +30,42 @@ FLAGS = [
 ]
 
 
+UNITS = ("lps.hip", "lps_table.hip", "lps_mx4head.hip")
+
+
+def _finish(cmd, proc) -> None:
+    out, err = proc.communicate()
+    if proc.returncode != 0:
+        raise RuntimeError(f"hipcc failed ({proc.returncode}):\n{' '.join(cmd)}\n{out}\n{err}")
+
+
+def _start(cmd):
+    return cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)
+
+
 def build(verbose: bool = False) -> str:
-    """Compile ``csrc/lps.hip`` into ``lps/liblps.so`` (always recompiles)."""
-    src = os.path.join(CSRC, "lps.hip")
+    """Compile the units of ``csrc`` into ``lps/liblps.so`` (always recompiles)."""
     tmp = OUT + ".tmp"
-    cmd = [HIPCC, *FLAGS, "-I", INCLUDE, "-I", CSRC, "-o", tmp, src]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"hipcc failed ({r.returncode}):\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    with tempfile.TemporaryDirectory() as objs:
+        made = [os.path.join(objs, u + ".o") for u in UNITS]
+        cmds = [[HIPCC, *FLAGS, "-I", INCLUDE, "-I", CSRC, "-c", os.path.join(CSRC, u), "-o", o]
+                for u, o in zip(UNITS, made)]
+        running = [_start(c) for c in cmds]
+        try:
+            for cmd, proc in running:
+                _finish(cmd, proc)
+        finally:
+            for _, proc in running:
+                if proc.poll() is None:
+                    proc.kill()
+                    proc.communicate()
+        link = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", tmp, *made]
+        _finish(*_start(link))
+        cmds.append(link)
     os.replace(tmp, OUT)
     if verbose:
-        print(" ".join(cmd))
+        for cmd in cmds:
+            print(" ".join(cmd))
     return OUT
 
 

@@ -17,15 +17,22 @@ import torch
 
 from . import _device as D
 from . import _lib
+from .vocab_table import Mx4Tensor
 
 
-def lm_head(hidden: torch.Tensor, weight: torch.Tensor, out_dtype: Optional[torch.dtype] = None,
+def lm_head(hidden: Union[torch.Tensor, Mx4Tensor], weight: Union[torch.Tensor, Mx4Tensor], out_dtype: Optional[torch.dtype] = None,
             return_stats: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """``hidden [..., H] @ weight[V, H].T`` -> logits ``[..., V]`` (fp32
     accumulation, stored in ``out_dtype``, default the input dtype).  Inputs:
     bf16 or fp16, the same dtype, ``H`` a multiple of 16.  ``return_stats``
     also returns ``[..., ceil(V / 128), 2]`` float32 block statistics
-    ``(max, sum(exp(v - max)))`` of the stored logits."""
+    ``(max, sum(exp(v - max)))`` of the stored logits.
+
+    ``weight`` may be 4-bit (``mx4_quantize``): then ``H`` is any number,
+    ``hidden`` bf16, fp16 or 4-bit itself, and ``out_dtype`` bfloat16 by default
+    for 4-bit ``hidden``.  The products are exact and summed in fp32."""
+    if isinstance(weight, Mx4Tensor) or isinstance(hidden, Mx4Tensor):
+        return _lm_head_mx4(hidden, weight, out_dtype, return_stats)
     D.require_device(hidden, "hidden")
     D.require_device(weight, "weight")
     if weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
@@ -58,6 +65,67 @@ def lm_head(hidden: torch.Tensor, weight: torch.Tensor, out_dtype: Optional[torc
         with D.guard(hidden.device):
             rc = _lib.load().lps_lm_head(ctypes.byref(a), D.stream_of(hidden.device))
         _lib.check(rc, "lps_lm_head")
+    out = out.reshape(*lead, V)
+    if return_stats:
+        return out, stats.reshape(*lead, G, 2)
+    return out
+
+
+def _words(s: torch.Tensor) -> torch.Tensor:
+    """Scales with rows on 4-byte lines, as the kernel reads them."""
+    if s.data_ptr() % 4 == 0 and (s.shape[0] <= 1 or s.stride(0) % 4 == 0):
+        return s
+    n = s.shape[1]
+    out = torch.empty((s.shape[0], n + -n % 4), dtype=torch.uint8, device=s.device)[:, :n]
+    return out.copy_(s)
+
+
+def _lm_head_mx4(hidden, weight, out_dtype, return_stats):
+    if not isinstance(weight, Mx4Tensor):
+        raise TypeError("a 4-bit hidden state needs a 4-bit weight")
+    weight.check("weight")
+    if weight.codes.dim() != 2 or weight.codes.shape[0] < 1:
+        raise ValueError(f"weight [V, H] expected; got {tuple(weight.shape)}")
+    if isinstance(hidden, Mx4Tensor):
+        hidden.check("hidden")
+    else:
+        D.require_device(hidden, "hidden")
+        if hidden.dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError("hidden must be bfloat16, float16 or an Mx4Tensor")
+    H = weight.hidden
+    if hidden.shape[-1:] != (H,):
+        raise ValueError(f"hidden [..., H] and weight [V, H] expected; got {tuple(hidden.shape)}, {tuple(weight.shape)}")
+    if hidden.device != weight.device:
+        raise ValueError(f"hidden and weight are on different devices: {hidden.device}, {weight.device}")
+    w, ws = weight.rows()
+    ws = _words(ws)
+    lead, V = hidden.shape[:-1], w.shape[0]
+    a = _lib.LmHeadMx4Args()
+    if isinstance(hidden, Mx4Tensor):
+        x, xs = hidden.rows()
+        xs = _words(xs)
+        od = out_dtype or torch.bfloat16
+        a.dtype = _lib.LPS_DTYPE_MX4
+        a.x_scales, a.x_scales_stride = xs.data_ptr(), xs.stride(0)
+    else:
+        x = hidden.reshape(-1, H)
+        if (x.stride(1) != 1 and H > 1) or (x.shape[0] > 1 and (x.stride(0) % 8 or x.stride(0) < H)) or x.data_ptr() % 16:
+            x = torch.empty((x.shape[0], H + -H % 8), dtype=x.dtype, device=x.device)[:, :H].copy_(x)
+        od = out_dtype or hidden.dtype
+        a.dtype = D.dtype_code(x)
+    M = x.shape[0]
+    out = torch.empty((M, V), dtype=od, device=w.device)
+    G = (V + _lib.LMHEAD_BLOCK_COLS - 1) // _lib.LMHEAD_BLOCK_COLS
+    stats = torch.empty((M, G, 2), dtype=torch.float32, device=w.device) if return_stats else None
+    a.out_dtype = D.dtype_code(out)
+    if M:
+        a.x, a.w, a.w_scales, a.out = x.data_ptr(), w.data_ptr(), ws.data_ptr(), out.data_ptr()
+        a.stats = D.ptr(stats)
+        a.rows, a.vocab, a.hidden = M, V, H
+        a.x_stride, a.w_stride, a.w_scales_stride, a.out_stride = x.stride(0), w.stride(0), ws.stride(0), V
+        with D.guard(w.device):
+            rc = _lib.load().lps_lm_head_mx4(ctypes.byref(a), D.stream_of(w.device))
+        _lib.check(rc, "lps_lm_head_mx4")
     out = out.reshape(*lead, V)
     if return_stats:
         return out, stats.reshape(*lead, G, 2)
