@@ -391,7 +391,8 @@ int lps_mx4_dequantize(const lps_mx4_args* args, void* stream);
 /* LM head over a 4-bit weight, lps_lm_head otherwise (logits, statistics):
  * x in bf16, fp16 or 4 bits.  Any hidden; the codes of w past a row's end count
  * as zeros, those of a 4-bit x must be (lps_mx4_quantize leaves them so).
- * Rows of x and w begin on 16-byte lines, rows of scales on 4-byte lines. */
+ * Rows of x and w begin on 16-byte lines, rows of scales on 4-byte lines;
+ * strides are at most 8 MiB. */
 typedef struct lps_lm_head_mx4_args {
   const void* x;                  /* [rows, hidden] in dtype; 4-bit codes */
   const void* x_scales;           /* 4-bit x: uint8 [rows, ceil(hidden / 32)] */

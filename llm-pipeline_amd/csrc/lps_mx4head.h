@@ -30,51 +30,76 @@ struct Mx4HeadParams {
   const uint8_t* ws;         // scales of w, rows on 4-byte lines
   const uint8_t* xs;         // scales of a 4-bit x, rows on 4-byte lines
   int64_t ws_stride, xs_stride;
+  int wide;                  // rows of scales lie and end on 16-byte lines
 };
 
 // One workgroup of WM x WN waves computes a BM x BN tile; K is walked in stages of
 // NB blocks (32 NB values) through a ring of NS LDS buffers, filled by loads that
-// cost no registers (lps_lmhead.h).  A stage holds the x rows, the w rows (16
-// bytes a block, chunk c of row r at place c ^ f(r)), then the scales of both, 4
-// bytes a row.  XB: bytes of a block of x, 64 or 16.
-template <int BM_, int BN_, int WM_, int WN_, int NS_, int WPE_, int XB_>
+// cost no registers (lps_lmhead.h).  A stage holds the x rows, then the w rows (16
+// bytes a block, chunk c of row r at place c ^ f(r)).  XB: bytes of a block of x,
+// 64 or 16.  A row has 4 bytes of scales where it has 64 of codes: loaded by the
+// stage they cost as many cache lines as the codes do (2048 x 4096 -> 151936 in 4
+// bits 1112 us, 732 without them), so that they come 32 blocks at a time, into two
+// buffers of their own.
+constexpr int M4_SB = 32;
+constexpr int64_t M4_MAX_STRIDE = 1 << 23;   // bytes: 256 rows of it fit 32-bit offsets
+template <int BM_, int BN_, int WM_, int WN_, int NB_, int NS_, int WPE_, int XB_>
 struct M4Tile {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NS = NS_, WPE = WPE_, XB = XB_;
-  static constexpr int NB = 4;                                  // blocks per stage
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NB = NB_, NS = NS_, WPE = WPE_, XB = XB_;
   static constexpr int NW = WM * WN, NT = 64 * NW;
   static constexpr int MT = BM / WM / 32, CT = BN / WN / 32;    // accumulators per wave: rows x columns
   static constexpr int WTN = 32 * CT;
   static constexpr int XC = NB * XB / 16, WC = NB;              // 16-byte chunks per row
   static constexpr int XRI = 64 / XC, WRI = 64 / WC;            // rows a wave's load instruction covers
-  static constexpr int XI = BM / XRI, WI = BN / WRI;             // load instructions of a stage
+  static constexpr int XI = BM / XRI, WI = BN / WRI;            // load instructions of a stage
   static constexpr int XPW = (XI + NW - 1) / NW, WPW = WI / NW; // ... of a wave (with more waves than XI some load the same)
   static constexpr bool XS = XB == 16;
-  static constexpr int SMR = BM < 64 ? 64 : BM;                 // scale rows of x a stage holds
-  static constexpr int LPW = XPW + WPW + 1 + (XS ? 1 : 0);      // loads per wave and stage
+  static constexpr int SROWS = BN + (XS ? BM : 0);              // rows with scales: w's, then x's
+  static constexpr int LPW = XPW + WPW;
   static constexpr int XBYTES = BM * XC * 16, WBYTES = BN * WC * 16;
-  static constexpr int STAGE = XBYTES + WBYTES + BN * 4 + (XS ? SMR * 4 : 0);
+  static constexpr int STAGE = XBYTES + WBYTES;
+  static constexpr int SBYTES = SROWS * M4_SB;
   static constexpr int KS = NB / 2;                             // steps of two blocks
+  static constexpr int PER = M4_SB / NB;                        // stages to a buffer of scales
+  static_assert(NB == 4 || NB == 8, "chunk places");
   static_assert((XI % NW == 0 || NW % XI == 0) && WI % NW == 0, "whole load instructions per wave");
-  static_assert(BN / 64 <= NW && SMR / 64 <= NW, "a load of scales per wave covers the tile");
+  static_assert(BN % 32 == 0 && BM % 32 == 0, "whole loads of scales");
   static_assert(BM % (32 * WM) == 0 && BN % (32 * WN) == 0 && BN % LMH_BN == 0, "tile shape");
-  static_assert((NS - 1) * LPW < 64, "the load counter holds 63");
+  static_assert(PER >= NS - 1, "scales are asked for before the stage that needs them");
+  static_assert((NS - 1) * LPW + 4 * SROWS / 32 / NW + 1 < 64, "the load counter holds 63");
   __device__ __forceinline__ static int xperm(int row) { return XC >= 8 ? (row & 7) : ((row >> 1) & 3); }
-  __device__ __forceinline__ static int wperm(int row) { return (row >> 1) & 3; }
+  __device__ __forceinline__ static int wperm(int row) { return WC >= 8 ? (row & 7) : ((row >> 1) & 3); }
 };
 template <typename T, int ES>
 constexpr int m4_lds_bytes() {
-  return T::NS * T::STAGE > lmh_epi_bytes<T, ES>() ? T::NS * T::STAGE : lmh_epi_bytes<T, ES>();
+  return T::NS * T::STAGE + 2 * T::SBYTES > lmh_epi_bytes<T, ES>() ? T::NS * T::STAGE + 2 * T::SBYTES : lmh_epi_bytes<T, ES>();
 }
 
 #ifndef LPS_HOST_EMU
-// 4 bytes per lane from g to LDS at (wave-uniform) base + 4 * lane.
-__device__ __forceinline__ void lmh_dma4(const char* g, char* base) {
-  const uint32_t m0 = (uint32_t)__builtin_amdgcn_readfirstlane(
-      (int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)base);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(m0), "v"(g) : "memory", "m0");
+// Byte address in LDS of a shared array.
+__device__ __forceinline__ uint32_t m4_lds(const char* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+}
+// 16 / 4 bytes per lane from base + off (base uniform) to LDS at (uniform) dst + 16 / 4 * lane.
+template <bool NTL>
+__device__ __forceinline__ void m4_dma16(const char* base, uint32_t off, uint32_t dst) {
+  if constexpr (NTL)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(dst), "v"(off), "s"(base) : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(off), "s"(base) : "memory");
+}
+__device__ __forceinline__ void m4_dma4(const char* base, uint32_t off, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(dst), "v"(off), "s"(base) : "memory");
 }
 #else
-inline void lmh_dma4(const char* g, char* base) { memcpy(base + 4 * ((int)threadIdx.x & 63), g, 4); }
+inline uint64_t m4_lds(const char* p) { return (uint64_t)(uintptr_t)p; }
+template <bool NTL>
+inline void m4_dma16(const char* base, uint32_t off, uint64_t dst) {
+  memcpy(reinterpret_cast<char*>(dst) + 16 * ((int)threadIdx.x & 63), base + off, 16);
+}
+inline void m4_dma4(const char* base, uint32_t off, uint64_t dst) {
+  memcpy(reinterpret_cast<char*>(dst) + 4 * ((int)threadIdx.x & 63), base + off, 4);
+}
 #endif
 
 // Eight codes as one fragment of the 16-bit instruction.
@@ -123,97 +148,76 @@ __device__ __forceinline__ bool m4_far_scale(uint32_t w) {
   return far;
 }
 
-// The accumulators plus one stage of NB blocks.
-template <int XDT, typename T, typename ACC>
-__device__ __forceinline__ void m4_stage(const char* stage, ACC (&acc)[T::MT][T::CT], int wm, int wn, int l, int steps) {
-  constexpr int MT = T::MT, CT = T::CT;
-  const int half = l >> 5;
-  const int xr = wm * (MT * 32) + (l & 31), wr = wn * T::WTN + (l & 31);
-  const int px = T::xperm(xr), pw = T::wperm(wr);   // (rows 32 apart share it)
-  const char* wb = stage + T::XBYTES;
-  const uint32_t* ws = reinterpret_cast<const uint32_t*>(wb + T::WBYTES);
-  uint32_t sw[CT];
+// The position of a lane in a tile, and its reads of a stage.
+template <typename T>
+struct M4Lane {
+  int half, xr, wr, px, pw;
+  __device__ __forceinline__ M4Lane(int wm, int wn, int l)
+      : half(l >> 5), xr(wm * (T::MT * 32) + (l & 31)), wr(wn * T::WTN + (l & 31)), px(T::xperm(xr)), pw(T::wperm(wr)) {}
+  // (rows 32 apart share their permutation)
+  __device__ __forceinline__ u32x4 x(const char* stage, int i, int c) const {
+    return *reinterpret_cast<const u32x4*>(stage + ((xr + 32 * i) * T::XC + (c ^ px)) * 16);
+  }
+  __device__ __forceinline__ u32x4 w(const char* stage, int i, int c) const {
+    return *reinterpret_cast<const u32x4*>(stage + T::XBYTES + ((wr + 32 * i) * T::WC + (c ^ pw)) * 16);
+  }
+  // four blocks' scales of a row (word d of the stage); this lane's are in bytes 0 and 2
+  __device__ __forceinline__ uint32_t ws_all(const char* scales, int i, int d) const {
+    return *reinterpret_cast<const uint32_t*>(scales + (wr + 32 * i) * M4_SB + 4 * d);
+  }
+  __device__ __forceinline__ uint32_t ws(const char* scales, int i, int d) const { return ws_all(scales, i, d) >> (8 * half); }
+  __device__ __forceinline__ uint32_t xs(const char* scales, int i, int d) const {
+    return *reinterpret_cast<const uint32_t*>(scales + (T::BN + xr + 32 * i) * M4_SB + 4 * d) >> (8 * half);
+  }
+};
+
+// A byte of a word of scales as the conversions' scale: its neighbours land in the
+// sign and the mantissa, which they ignore.
+__device__ __forceinline__ float m4_scale(uint32_t w, int j) { return __uint_as_float((j & 1) ? w << 7 : w << 23); }
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ i32x8 m4_operand(u32x4 v) { return i32x8{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0}; }
+template <typename ACC>
+__device__ __forceinline__ ACC m4_mma4(u32x4 a, u32x4 b, ACC c, uint32_t sa, uint32_t sb, int j) {
+  if (j & 1) return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(m4_operand(a), m4_operand(b), c, 4, 4, 2, (int)sa, 2, (int)sb);
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(m4_operand(a), m4_operand(b), c, 4, 4, 0, (int)sa, 0, (int)sb);
+}
+
+// The accumulators plus `steps` steps of two blocks, one after another: the last
+// columns of a row, and (FAR) stages of fp16 with scales that it does not hold.
+template <int XDT, typename T, bool FAR, typename ACC>
+__device__ __forceinline__ void m4_plain_stage(const char* stage, const char* scales, const M4Lane<T>& L,
+                                               ACC (&acc)[T::MT][T::CT], int steps) {
+#pragma unroll 1
+  for (int j = 0; j < steps; j++) {
+    const int c = 2 * j + L.half;
 #pragma unroll
-  for (int i = 0; i < CT; i++) sw[i] = ws[wr + 32 * i];
-  if constexpr (T::XS) {
-    const uint32_t* xs = ws + T::BN;
-    uint32_t sx[MT];
+    for (int b = 0; b < T::CT; b++) {
+      const u32x4 cw = L.w(stage, b, c);
+      const uint32_t byte = (L.ws_all(scales, b, j >> 1) >> (8 * (c & 3))) & 255u;
+      if constexpr (T::XS) {
 #pragma unroll
-    for (int i = 0; i < MT; i++) sx[i] = xs[xr + 32 * i] >> (8 * half);
-#pragma unroll
-    for (int i = 0; i < CT; i++) sw[i] >>= 8 * half;
-#pragma unroll
-    for (int j = 0; j < T::KS; j++) {
-      if (j >= steps) break;
-      typedef int i32x8 __attribute__((ext_vector_type(8)));
-      const int c = 2 * j + half;
-      u32x4 fx[MT], fw[CT];
-#pragma unroll
-      for (int i = 0; i < MT; i++) fx[i] = *reinterpret_cast<const u32x4*>(stage + ((xr + 32 * i) * T::XC + (c ^ px)) * 16);
-#pragma unroll
-      for (int i = 0; i < CT; i++) fw[i] = *reinterpret_cast<const u32x4*>(wb + ((wr + 32 * i) * T::WC + (c ^ pw)) * 16);
-#pragma unroll
-      for (int a = 0; a < MT; a++)
-#pragma unroll
-        for (int b = 0; b < CT; b++) {
-          const i32x8 A = {(int)fx[a].x, (int)fx[a].y, (int)fx[a].z, (int)fx[a].w, 0, 0, 0, 0};
-          const i32x8 B = {(int)fw[b].x, (int)fw[b].y, (int)fw[b].z, (int)fw[b].w, 0, 0, 0, 0};
-          if (j == 0)
-            acc[a][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, B, acc[a][b], 4, 4, 0, (int)sx[a], 0, (int)sw[b]);
-          else
-            acc[a][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, B, acc[a][b], 4, 4, 2, (int)sx[a], 2, (int)sw[b]);
-        }
-    }
-  } else {
-    bool far = false;
-    if constexpr (XDT == LPS_DTYPE_F16) {
-#pragma unroll
-      for (int i = 0; i < CT; i++) far = far || m4_far_scale(sw[i]);
-      far = wballot(far) != 0;
-    }
-#pragma unroll
-    for (int j = 0; j < T::KS; j++) {
-      if (j >= steps) break;
-      const int c = 2 * j + half;
-      u32x4 cw[CT];
-      float s[CT];
-#pragma unroll
-      for (int i = 0; i < CT; i++) {
-        cw[i] = *reinterpret_cast<const u32x4*>(wb + ((wr + 32 * i) * T::WC + (c ^ pw)) * 16);
-        s[i] = __uint_as_float(((sw[i] >> (8 * c)) & 255u) << 23);
-      }
-      auto step = [&](auto far_c) {
-        constexpr bool FAR = decltype(far_c)::value;
+        for (int a = 0; a < T::MT; a++)
+          acc[a][b] = m4_mma4(L.x(stage, a, c), cw, acc[a][b], L.xs(scales, a, j >> 1) >> (16 * (j & 1)), byte, 0);
+      } else {
+        const float s = __uint_as_float(byte << 23);
 #pragma unroll
         for (int q = 0; q < 4; q++) {
-          u32x4 fx[MT];
+          const u32x4 fw = m4_frag<FAR ? LPS_DTYPE_BF16 : XDT>(cw[q], s);
 #pragma unroll
-          for (int i = 0; i < MT; i++)
-            fx[i] = *reinterpret_cast<const u32x4*>(stage + ((xr + 32 * i) * T::XC + ((4 * c + q) ^ px)) * 16);
-          if constexpr (!FAR) {
-#pragma unroll
-            for (int b = 0; b < CT; b++) {
-              const u32x4 fw = m4_frag<XDT>(cw[b][q], s[b]);
-#pragma unroll
-              for (int a = 0; a < MT; a++) acc[a][b] = MfmaOps<XDT>::mma(fx[a], fw, acc[a][b]);
-            }
-          } else {
-#pragma unroll
-            for (int a = 0; a < MT; a++) {
+          for (int a = 0; a < T::MT; a++) {
+            const u32x4 fx = L.x(stage, a, 4 * c + q);
+            if constexpr (FAR) {
               u32x4 hi, lo;
-              m4_split(fx[a], hi, lo);
-#pragma unroll
-              for (int b = 0; b < CT; b++) {
-                const u32x4 fw = m4_frag<LPS_DTYPE_BF16>(cw[b][q], s[b]);
-                acc[a][b] = MfmaOps<LPS_DTYPE_BF16>::mma(hi, fw, acc[a][b]);
-                acc[a][b] = MfmaOps<LPS_DTYPE_BF16>::mma(lo, fw, acc[a][b]);
-              }
+              m4_split(fx, hi, lo);
+              acc[a][b] = MfmaOps<LPS_DTYPE_BF16>::mma(hi, fw, acc[a][b]);
+              acc[a][b] = MfmaOps<LPS_DTYPE_BF16>::mma(lo, fw, acc[a][b]);
+            } else {
+              acc[a][b] = MfmaOps<XDT>::mma(fx, fw, acc[a][b]);
             }
           }
         }
-      };
-      if (XDT == LPS_DTYPE_F16 && far) step(std::true_type{});
-      else step(std::false_type{});
+      }
     }
   }
 }
@@ -223,7 +227,7 @@ template <int XDT, int ODT, typename T, bool NTL>
 __global__ __launch_bounds__(T::NT, T::WPE) void mx4head_kernel(Mx4HeadParams Q) {
   constexpr int ES = ODT == LPS_DTYPE_F32 ? 4 : 2;
   constexpr int ADT = XDT == LPS_DTYPE_F16 ? LPS_DTYPE_F16 : LPS_DTYPE_BF16;   // (the accumulators are alike)
-  constexpr int MT = T::MT, CT = T::CT, NB = T::NB;
+  constexpr int MT = T::MT, CT = T::CT, NB = T::NB, KS = T::KS;
   __shared__ __attribute__((aligned(1024))) char lds[m4_lds_bytes<T, ES>()];
   const LmHeadParams& P = Q.h;
   // tiles over the XCDs as in lmhead_kernel: a run each, the row tiles of one column tile first
@@ -231,77 +235,188 @@ __global__ __launch_bounds__(T::NT, T::WPE) void mx4head_kernel(Mx4HeadParams Q)
   const int t = ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);
   if (((int)blockIdx.x >> 3) >= per || t >= P.tiles) return;   // uniform over the workgroup
   const int m0 = (t % P.mtiles) * T::BM, n0 = (t / P.mtiles) * T::BN;
-  const int wv = (int)threadIdx.x >> 6, l = (int)threadIdx.x & 63;
+  const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), l = (int)threadIdx.x & 63;
   const int wm = wv / T::WN, wn = wv % T::WN;
-  auto mrow = [&](int r) { const int m = m0 + r; return (int64_t)(m < P.M ? m : P.M - 1); };
-  auto nrow = [&](int r) { const int n = n0 + r; return (int64_t)(n < P.V ? n : P.V - 1); };
-  const char* const X = reinterpret_cast<const char*>(P.x);
-  const char* const W = reinterpret_cast<const char*>(P.w);
   const int64_t xstep = T::XS ? P.x_stride : 2 * P.x_stride;   // bytes of a row of x
+  const char* const X = reinterpret_cast<const char*>(P.x) + (int64_t)m0 * xstep;
+  const char* const W = reinterpret_cast<const char*>(P.w) + (int64_t)n0 * P.w_stride;
+  // rows of the tile, clamped into range (the others' results are dropped); their
+  // offsets in it fit 32 bits (M4_MAX_STRIDE)
+  auto mrow = [&](int r) { return m0 + r < P.M ? r : P.M - 1 - m0; };
+  auto nrow = [&](int r) { return n0 + r < P.V ? r : P.V - 1 - n0; };
 
-  // sources of this lane's chunks (rows clamped into range; their results are dropped)
-  const char* xsrc[T::XPW];
-  const char* wsrc[T::WPW];
+  uint32_t xoff[T::XPW], woff[T::WPW];
 #pragma unroll
   for (int i = 0; i < T::XPW; i++) {
     const int row = ((i * T::NW + wv) % T::XI) * T::XRI + l / T::XC, c = (l % T::XC) ^ T::xperm(row);
-    xsrc[i] = X + mrow(row) * xstep + c * 16;
+    xoff[i] = (uint32_t)mrow(row) * (uint32_t)xstep + c * 16;
   }
 #pragma unroll
   for (int i = 0; i < T::WPW; i++) {
     const int row = (i * T::NW + wv) * T::WRI + l / T::WC, c = (l % T::WC) ^ T::wperm(row);
-    wsrc[i] = W + nrow(row) * P.w_stride + c * 16;
+    woff[i] = (uint32_t)nrow(row) * (uint32_t)P.w_stride + c * 16;
   }
-  // (with more waves than groups of 64 rows some load the same scales)
-  const int sg = wv % (T::BN / 64), xg = wv % (T::SMR / 64);
-  const char* ssrc = reinterpret_cast<const char*>(Q.ws) + nrow(64 * sg + l) * Q.ws_stride;
-  const char* xssrc = T::XS ? reinterpret_cast<const char*>(Q.xs) + mrow(64 * xg + l) * Q.xs_stride : nullptr;
-  auto issue = [&](int buf) {   // the next stage into ring buffer buf
-    char* base = lds + buf * T::STAGE;
+  const auto lds0 = m4_lds(lds);
+  auto issue = [&](int s, int buf) {   // stage s into ring buffer buf
+    const char* xb = X + (int64_t)s * (NB * T::XB);
+    const char* wb = W + (int64_t)s * (NB * 16);
+    const auto d = lds0 + buf * T::STAGE;
 #pragma unroll
-    for (int i = 0; i < T::XPW; i++) {
-      lmh_dma16<false>(xsrc[i], base + ((i * T::NW + wv) % T::XI) * 1024);
-      xsrc[i] += NB * T::XB;
-    }
-    base += T::XBYTES;
+    for (int i = 0; i < T::XPW; i++) m4_dma16<false>(xb, xoff[i], d + ((i * T::NW + wv) % T::XI) * 1024);
 #pragma unroll
-    for (int i = 0; i < T::WPW; i++) {
-      lmh_dma16<NTL>(wsrc[i], base + (i * T::NW + wv) * 1024);
-      wsrc[i] += NB * 16;
-    }
-    base += T::WBYTES;
-    lmh_dma4(ssrc, base + sg * 256);
-    ssrc += NB;
-    if constexpr (T::XS) {
-      lmh_dma4(xssrc, base + T::BN * 4 + xg * 256);
-      xssrc += NB;
+    for (int i = 0; i < T::WPW; i++) m4_dma16<NTL>(wb, woff[i], d + T::XBYTES + (i * T::NW + wv) * 1024);
+  };
+  const int ns = P.H / (32 * NB);   // whole stages of whole blocks; the rest of H follows them
+  // scales of blocks 32 u .. +31, as far as the whole stages go: a row's 32 bytes
+  // by two lanes, or by eight where it does not lie on 16-byte lines
+  char* const sbuf = lds + T::NS * T::STAGE;
+  const auto sdst = lds0 + T::NS * T::STAGE;
+  const char* const WS = reinterpret_cast<const char*>(Q.ws) + (int64_t)n0 * Q.ws_stride;
+  const char* const XSC = T::XS ? reinterpret_cast<const char*>(Q.xs) + (int64_t)m0 * Q.xs_stride : nullptr;
+  auto issue_scales = [&](int u) {
+    const auto d = sdst + (u & 1) * T::SBYTES;
+    const int rl = Q.wide ? 32 : 8, groups = T::SROWS / rl, r0 = Q.wide ? l >> 1 : l >> 3;
+    int b = M4_SB * u + (Q.wide ? 16 * (l & 1) : 4 * (l & 7));
+    b = b < NB * ns ? b : 0;          // (a row without them: others of its own)
+    for (int i = wv; i < groups; i += T::NW) {
+      const bool ofx = T::XS && rl * i >= T::BN;
+      const char* base = ofx ? XSC : WS;
+      const uint32_t off = (ofx ? (uint32_t)mrow(rl * i + r0 - T::BN) * (uint32_t)Q.xs_stride
+                                : (uint32_t)nrow(rl * i + r0) * (uint32_t)Q.ws_stride) + b;
+      if (Q.wide) m4_dma16<false>(base, off, d + i * 1024);
+      else m4_dma4(base, off, d + i * 256);
     }
   };
 
   typename MfmaOps<ADT>::acc acc[MT][CT] = {};
-  const int ns = P.H / (32 * NB);   // whole stages of whole blocks; the rest of H follows them
-  for (int s = 0; s < T::NS - 1 && s < ns; s++) issue(s);
-  int buf = 0;
-  for (int s = 0; s < ns; s++) {
-    // stage s has landed, and every wave is done with stage s - 1
-    lmh_wait_stage<T>(ns - 1 - s);
-    if (s + T::NS - 1 < ns) issue(buf == 0 ? T::NS - 1 : buf - 1);
-    m4_stage<XDT, T>(lds + buf * T::STAGE, acc, wm, wn, l, T::KS);
-    buf = buf + 1 == T::NS ? 0 : buf + 1;
+  const M4Lane<T> L(wm, wn, l);
+  // Fragments are read one step ahead of their matrix instructions and, of a
+  // 16-bit x, the codes converted one ahead, in the shadow of the matrix cores;
+  // the last step of a stage waits for the next one and reads its first.
+  constexpr int STEPS = T::XS ? KS : 4 * KS;       // matrix steps of a stage (64 or 16 values)
+  u32x4 fx[2][MT], cw[2][CT], fw[2][CT];
+  uint32_t sw[NB / 4][CT], sx[NB / 4][MT];
+  auto read_scales = [&](const char* scales) {
+#pragma unroll
+    for (int d = 0; d < NB / 4; d++) {
+#pragma unroll
+      for (int i = 0; i < CT; i++) sw[d][i] = L.ws(scales, i, d);
+      if constexpr (T::XS) {
+#pragma unroll
+        for (int i = 0; i < MT; i++) sx[d][i] = L.xs(scales, i, d);
+      }
+    }
+  };
+  auto read_x = [&](const char* stage, int k) {    // for matrix step k
+    const int c = T::XS ? 2 * k + L.half : 4 * (2 * (k >> 2) + L.half) + (k & 3);
+#pragma unroll
+    for (int i = 0; i < MT; i++) fx[k & 1][i] = L.x(stage, i, c);
+  };
+  auto read_w = [&](const char* stage, int j) {    // for blocks 2 j and 2 j + 1
+#pragma unroll
+    for (int i = 0; i < CT; i++) cw[j & 1][i] = L.w(stage, i, 2 * j + L.half);
+  };
+  auto convert = [&](int k) {
+    if constexpr (!T::XS) {
+      const int j = k >> 2;
+#pragma unroll
+      for (int i = 0; i < CT; i++) fw[k & 1][i] = m4_frag<XDT>(cw[j & 1][i][k & 3], m4_scale(sw[j >> 1][i], j));
+    }
+  };
+  auto far_scales = [&](const char* scales) {      // (uniform over the wave)
+    bool far = false;
+    if constexpr (XDT == LPS_DTYPE_F16) {
+#pragma unroll
+      for (int d = 0; d < NB / 4; d++)
+#pragma unroll
+        for (int i = 0; i < CT; i++) far = far || m4_far_scale(L.ws_all(scales, i, d));
+      far = wballot(far) != 0;
+    }
+    return far;
+  };
+  auto scales_of = [&](int s) { return sbuf + ((s / T::PER) & 1) * T::SBYTES + (s % T::PER) * NB; };
+  if (ns > 0) {
+    issue_scales(0);
+    for (int s = 0; s < T::NS && s < ns; s++) issue(s, s);
+    if (ns >= T::NS) lmh_wait_barrier<(T::NS - 1) * T::LPW>();
+    else lmh_wait_barrier<0>();
+    read_scales(scales_of(0));
+    read_w(lds, 0);
+    read_x(lds, 0);
+    convert(0);
+    int buf = 0;
+    for (int s = 0; s < ns; s++) {
+      const char* cur = lds + buf * T::STAGE;
+      const int nb = buf + 1 == T::NS ? 0 : buf + 1;
+      const bool far = far_scales(scales_of(s));
+      if (XDT == LPS_DTYPE_F16 && far) m4_plain_stage<XDT, T, true>(cur, scales_of(s), L, acc, KS);
+#pragma unroll
+      for (int k = 0; k < STEPS; k++) {
+        if (k + 1 < STEPS) {
+          if (XDT == LPS_DTYPE_F16 && far) continue;
+          if constexpr (T::XS) read_w(cur, k + 1);
+          else if ((k & 3) == 1 && (k >> 2) + 1 < KS) read_w(cur, (k >> 2) + 1);
+          read_x(cur, k + 1);
+          __builtin_amdgcn_sched_barrier(0);   // (the compiler would move the reads down to their use)
+        }
+        if (k + 1 == STEPS) {
+          uint32_t ow[CT], ox[MT];   // (this step's scales)
+          if constexpr (T::XS) {
+#pragma unroll
+            for (int i = 0; i < CT; i++) ow[i] = sw[NB / 4 - 1][i];
+#pragma unroll
+            for (int i = 0; i < MT; i++) ox[i] = sx[NB / 4 - 1][i];
+          }
+          if (s + 1 < ns) {
+            // every wave holds its last fragments of stage s, stage s + 1 has landed
+            // (and its scales, asked for before it)
+            lmh_wait_stage<T>(ns - 2 - s);
+            if (s % T::PER == 0 && s + T::PER < ns) issue_scales(s / T::PER + 1);
+            if (s + T::NS < ns) issue(s + T::NS, buf);
+            read_scales(scales_of(s + 1));
+            read_w(lds + nb * T::STAGE, 0);
+            read_x(lds + nb * T::STAGE, 0);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          if (!(XDT == LPS_DTYPE_F16 && far)) {
+#pragma unroll
+            for (int a = 0; a < MT; a++)
+#pragma unroll
+              for (int b = 0; b < CT; b++) {
+                if constexpr (T::XS) acc[a][b] = m4_mma4(fx[k & 1][a], cw[k & 1][b], acc[a][b], ox[a], ow[b], k);
+                else acc[a][b] = MfmaOps<ADT>::mma(fx[k & 1][a], fw[k & 1][b], acc[a][b]);
+              }
+          }
+          if (s + 1 < ns) convert(0);
+        } else {
+#pragma unroll
+          for (int a = 0; a < MT; a++)
+#pragma unroll
+            for (int b = 0; b < CT; b++) {
+              if constexpr (T::XS) acc[a][b] = m4_mma4(fx[k & 1][a], cw[k & 1][b], acc[a][b], sx[k >> 1][a], sw[k >> 1][b], k);
+              else acc[a][b] = MfmaOps<ADT>::mma(fx[k & 1][a], fw[k & 1][b], acc[a][b]);
+            }
+          convert(k + 1);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      buf = nb;
+    }
+    __syncthreads();
   }
-  lmh_wait_barrier<0>();
   const int k0 = ns * 32 * NB;
   if (k0 < P.H) {
     // the columns past the last whole stage, zeros up to one (with scales of 1)
-    const int nb = (P.H + 31) >> 5, b0 = ns * NB;
+    const int nblk = (P.H + 31) >> 5, b0 = ns * NB;
     for (int i = threadIdx.x; i < T::BM * T::XC; i += T::NT) {
       const int row = i / T::XC, c = (i % T::XC) ^ T::xperm(row);
       u32x4 v = {0u, 0u, 0u, 0u};
+      const char* xr = X + (int64_t)mrow(row) * xstep;
       if constexpr (T::XS) {
-        if (b0 + c < nb) v = *reinterpret_cast<const u32x4*>(X + mrow(row) * xstep + (b0 + c) * 16);
+        if (b0 + c < nblk) v = *reinterpret_cast<const u32x4*>(xr + (b0 + c) * 16);
       } else {
         const int e0 = k0 + 8 * c;
-        if (e0 < P.H) v = load_piece<ADT>(X + mrow(row) * xstep, e0, P.H).q[0];
+        if (e0 < P.H) v = load_piece<ADT>(xr, e0, P.H).q[0];
       }
       *reinterpret_cast<u32x4*>(lds + i * 16) = v;
     }
@@ -309,8 +424,8 @@ __global__ __launch_bounds__(T::NT, T::WPE) void mx4head_kernel(Mx4HeadParams Q)
     for (int i = threadIdx.x; i < T::BN * T::WC; i += T::NT) {
       const int row = i / T::WC, b = b0 + ((i % T::WC) ^ T::wperm(row));
       u32x4 v = {0u, 0u, 0u, 0u};
-      if (b < nb) {
-        v = *reinterpret_cast<const u32x4*>(W + nrow(row) * P.w_stride + b * 16);
+      if (b < nblk) {
+        v = *reinterpret_cast<const u32x4*>(W + (int64_t)nrow(row) * P.w_stride + b * 16);
 #pragma unroll
         for (int e = 0; e < 4; e++) {               // (codes past the row's end count as zeros, whatever they hold)
           const int keep = P.H - 32 * b - 8 * e;
@@ -319,14 +434,17 @@ __global__ __launch_bounds__(T::NT, T::WPE) void mx4head_kernel(Mx4HeadParams Q)
       }
       *reinterpret_cast<u32x4*>(wb + i * 16) = v;
     }
-    uint8_t* sb = reinterpret_cast<uint8_t*>(wb + T::WBYTES);
-    for (int i = threadIdx.x; i < T::BN * NB; i += T::NT)
-      sb[i] = b0 + i % NB < nb ? Q.ws[nrow(i / NB) * Q.ws_stride + b0 + i % NB] : 127;
-    if constexpr (T::XS)
-      for (int i = threadIdx.x; i < T::BM * NB; i += T::NT)
-        sb[T::BN * 4 + i] = b0 + i % NB < nb ? Q.xs[mrow(i / NB) * Q.xs_stride + b0 + i % NB] : 127;
+    for (int i = threadIdx.x; i < T::SROWS * NB; i += T::NT) {
+      const int row = i / NB, b = b0 + i % NB;
+      const char* sr = WS + (int64_t)nrow(row < T::BN ? row : 0) * Q.ws_stride;
+      if constexpr (T::XS)
+        if (row >= T::BN) sr = XSC + (int64_t)mrow(row - T::BN) * Q.xs_stride;
+      sbuf[row * M4_SB + i % NB] = b < nblk ? sr[b] : (char)127;
+    }
     __syncthreads();
-    m4_stage<XDT, T>(lds, acc, wm, wn, l, (nb - b0 + 1) / 2);
+    const int steps = (nblk - b0 + 1) / 2;
+    if (XDT == LPS_DTYPE_F16 && far_scales(sbuf)) m4_plain_stage<XDT, T, true>(lds, sbuf, L, acc, steps);
+    else m4_plain_stage<XDT, T, false>(lds, sbuf, L, acc, steps);
     __syncthreads();
   }
   lmh_epilogue<ADT, ODT, T>(P, lds, acc, n0, m0, wv, l);

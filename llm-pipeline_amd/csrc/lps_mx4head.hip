@@ -22,12 +22,12 @@ template <int XDT, int ODT>
 hipError_t launch_mx4head_rows(const Mx4HeadParams& Q, hipStream_t s) {
   constexpr int XB = XDT == DT_MX4 ? 16 : 64;
   switch (mx4head_shape(Q.h.M)) {
-    case 0: return launch_mx4head<XDT, ODT, M4Tile<32, 128, 1, 4, 6, 1, XB>, true>(Q, s);
-    case 1: return launch_mx4head<XDT, ODT, M4Tile<64, 128, 1, 4, 5, 1, XB>, true>(Q, s);
-    case 2: return launch_mx4head<XDT, ODT, M4Tile<128, 128, 4, 2, 3, 2, XB>, true>(Q, s);
+    case 0: return launch_mx4head<XDT, ODT, M4Tile<32, 128, 1, 4, 8, 3, 1, XB>, true>(Q, s);
+    case 1: return launch_mx4head<XDT, ODT, M4Tile<64, 128, 1, 4, 4, 4, 1, XB>, true>(Q, s);
+    case 2: return launch_mx4head<XDT, ODT, M4Tile<128, 128, 4, 2, 4, 3, 2, XB>, true>(Q, s);
     default:
-      if constexpr (XB == 16) return launch_mx4head<XDT, ODT, M4Tile<256, 256, 4, 2, 4, 2, XB>, false>(Q, s);
-      else return launch_mx4head<XDT, ODT, M4Tile<128, 256, 2, 4, 3, 2, XB>, false>(Q, s);
+      if constexpr (XB == 16) return launch_mx4head<XDT, ODT, M4Tile<256, 256, 4, 2, 4, 3, 2, XB>, false>(Q, s);
+      else return launch_mx4head<XDT, ODT, M4Tile<128, 256, 2, 2, 4, 2, 1, XB>, false>(Q, s);
   }
 }
 template <int XDT>
@@ -61,6 +61,9 @@ extern "C" int lps_lm_head_mx4(const lps_lm_head_mx4_args* a, void* stream) {
   if (a->rows > 1 && (P.x_stride < (x4 ? 16 * nb : a->hidden) || P.out_stride < a->vocab)) return LPS_EINVAL;
   if (a->vocab > 1 && (P.w_stride < 16 * nb || Q.ws_stride < nb)) return LPS_EINVAL;
   if (x4 && a->rows > 1 && Q.xs_stride < nb) return LPS_EINVAL;
+  if ((x4 ? 1 : 2) * P.x_stride > M4_MAX_STRIDE || P.w_stride > M4_MAX_STRIDE || Q.ws_stride > M4_MAX_STRIDE ||
+      Q.xs_stride > M4_MAX_STRIDE)
+    return LPS_EINVAL;
   // 16-byte operand loads, 4-byte loads of scales
   if (reinterpret_cast<uintptr_t>(a->x) % 16 || P.x_stride % (x4 ? 16 : 8) || reinterpret_cast<uintptr_t>(a->w) % 16 ||
       P.w_stride % 16)
@@ -77,6 +80,8 @@ extern "C" int lps_lm_head_mx4(const lps_lm_head_mx4_args* a, void* stream) {
   P.G = (a->vocab + LMH_BN - 1) / LMH_BN;
   Q.ws = static_cast<const uint8_t*>(a->w_scales);
   Q.xs = static_cast<const uint8_t*>(a->x_scales);
+  auto wide = [&](const void* p, int64_t stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 16 == 0; };
+  Q.wide = nb % 16 == 0 && wide(Q.ws, Q.ws_stride) && (!x4 || wide(Q.xs, Q.xs_stride));
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const hipError_t e = x4 ? dispatch_mx4head<DT_MX4>(Q, a->out_dtype, s)
                        : a->dtype == LPS_DTYPE_BF16 ? dispatch_mx4head<LPS_DTYPE_BF16>(Q, a->out_dtype, s)

@@ -31,6 +31,14 @@ def dtype_code(t: torch.Tensor) -> int:
         raise TypeError(f"unsupported logits dtype {t.dtype}; expected float32, bfloat16 or float16") from None
 
 
+def code_of(dtype: torch.dtype) -> int:
+    """``dtype_code`` of a type."""
+    code = _DTYPES.get(dtype)
+    if code is None:
+        raise TypeError(f"unsupported dtype {dtype}; expected float32, bfloat16 or float16")
+    return code
+
+
 def ptr(t) -> int:
     return 0 if t is None else int(t.data_ptr())
 

@@ -17,7 +17,9 @@ import torch
 
 from . import _device as D
 from . import _lib
-from .vocab_table import Mx4Tensor
+from .vocab_table import Mx4Tensor, _call, _on_gpu, _same_device
+
+_pack_mx4 = _lib.packer(_lib.LmHeadMx4Args)
 
 
 def lm_head(hidden: Union[torch.Tensor, Mx4Tensor], weight: Union[torch.Tensor, Mx4Tensor], out_dtype: Optional[torch.dtype] = None,
@@ -71,6 +73,9 @@ def lm_head(hidden: Union[torch.Tensor, Mx4Tensor], weight: Union[torch.Tensor, 
     return out
 
 
+_MX4_MAX_STRIDE = 1 << 23   # bytes between rows (include/lps.h)
+
+
 def _words(s: torch.Tensor) -> torch.Tensor:
     """Scales with rows on 4-byte lines, as the kernel reads them."""
     if s.data_ptr() % 4 == 0 and (s.shape[0] <= 1 or s.stride(0) % 4 == 0):
@@ -84,49 +89,44 @@ def _lm_head_mx4(hidden, weight, out_dtype, return_stats):
     if not isinstance(weight, Mx4Tensor):
         raise TypeError("a 4-bit hidden state needs a 4-bit weight")
     weight.check("weight")
-    if weight.codes.dim() != 2 or weight.codes.shape[0] < 1:
-        raise ValueError(f"weight [V, H] expected; got {tuple(weight.shape)}")
+    H = weight.hidden
     if isinstance(hidden, Mx4Tensor):
         hidden.check("hidden")
-    else:
-        D.require_device(hidden, "hidden")
-        if hidden.dtype not in (torch.bfloat16, torch.float16):
-            raise TypeError("hidden must be bfloat16, float16 or an Mx4Tensor")
-    H = weight.hidden
-    if hidden.shape[-1:] != (H,):
-        raise ValueError(f"hidden [..., H] and weight [V, H] expected; got {tuple(hidden.shape)}, {tuple(weight.shape)}")
-    if hidden.device != weight.device:
-        raise ValueError(f"hidden and weight are on different devices: {hidden.device}, {weight.device}")
-    w, ws = weight.rows()
-    ws = _words(ws)
-    lead, V = hidden.shape[:-1], w.shape[0]
-    a = _lib.LmHeadMx4Args()
-    if isinstance(hidden, Mx4Tensor):
+        code, od = _lib.LPS_DTYPE_MX4, out_dtype or torch.bfloat16
+        lead, width = hidden.codes.shape[:-1], hidden.hidden
         x, xs = hidden.rows()
         xs = _words(xs)
-        od = out_dtype or torch.bfloat16
-        a.dtype = _lib.LPS_DTYPE_MX4
-        a.x_scales, a.x_scales_stride = xs.data_ptr(), xs.stride(0)
+        xp, xss = xs.data_ptr(), xs.stride(0)
     else:
-        x = hidden.reshape(-1, H)
-        if (x.stride(1) != 1 and H > 1) or (x.shape[0] > 1 and (x.stride(0) % 8 or x.stride(0) < H)) or x.data_ptr() % 16:
-            x = torch.empty((x.shape[0], H + -H % 8), dtype=x.dtype, device=x.device)[:, :H].copy_(x)
-        od = out_dtype or hidden.dtype
-        a.dtype = D.dtype_code(x)
+        _on_gpu(hidden, "hidden")
+        if hidden.dtype is not torch.bfloat16 and hidden.dtype is not torch.float16:
+            raise TypeError("hidden must be bfloat16, float16 or an Mx4Tensor")
+        code, od = D.code_of(hidden.dtype), out_dtype or hidden.dtype
+        lead, width = hidden.shape[:-1], hidden.shape[-1] if hidden.dim() else 0
+        x, xp, xss = hidden, 0, 0
+        if x.dim() != 2 and width:
+            x = x.reshape(-1, width)
+    if width != H or weight.codes.dim() != 2 or weight.codes.shape[0] < 1:
+        raise ValueError(f"hidden [..., H] and weight [V, H] expected; got {tuple(hidden.shape)}, {tuple(weight.shape)}")
+    _same_device(x, weight.codes, "hidden and weight")
     M = x.shape[0]
-    out = torch.empty((M, V), dtype=od, device=w.device)
+    if code != _lib.LPS_DTYPE_MX4:
+        r, e = x.stride()
+        # rows on 16-byte lines: a copy that lies so
+        if (e != 1 and H > 1) or x.data_ptr() % 16 or (M > 1 and (r % 8 or not H <= r <= _MX4_MAX_STRIDE // 2)):
+            x = torch.empty((M, H + -H % 8), dtype=x.dtype, device=x.device)[:, :H].copy_(x)
+    w, ws = weight.rows()
+    ws = _words(ws)
+    device, V = w.device, w.shape[0]
+    out_code = D.code_of(od)
+    out = torch.empty((M, V), dtype=od, device=device)
     G = (V + _lib.LMHEAD_BLOCK_COLS - 1) // _lib.LMHEAD_BLOCK_COLS
-    stats = torch.empty((M, G, 2), dtype=torch.float32, device=w.device) if return_stats else None
-    a.out_dtype = D.dtype_code(out)
+    stats = torch.empty((M, G, 2), dtype=torch.float32, device=device) if return_stats else None
     if M:
-        a.x, a.w, a.w_scales, a.out = x.data_ptr(), w.data_ptr(), ws.data_ptr(), out.data_ptr()
-        a.stats = D.ptr(stats)
-        a.rows, a.vocab, a.hidden = M, V, H
-        a.x_stride, a.w_stride, a.w_scales_stride, a.out_stride = x.stride(0), w.stride(0), ws.stride(0), V
-        with D.guard(w.device):
-            rc = _lib.load().lps_lm_head_mx4(ctypes.byref(a), D.stream_of(w.device))
-        _lib.check(rc, "lps_lm_head_mx4")
-    out = out.reshape(*lead, V)
-    if return_stats:
-        return out, stats.reshape(*lead, G, 2)
-    return out
+        _call("lps_lm_head_mx4",
+              _pack_mx4(x.data_ptr(), xp, w.data_ptr(), ws.data_ptr(), out.data_ptr(), D.ptr(stats), code, out_code, M, V, H,
+                        x.stride(0), xss, w.stride(0), ws.stride(0), V), device)
+    if len(lead) != 1:
+        out = out.reshape(*lead, V)
+        stats = None if stats is None else stats.reshape(*lead, G, 2)
+    return (out, stats) if return_stats else out

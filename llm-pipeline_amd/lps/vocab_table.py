@@ -10,7 +10,6 @@ form in microscaled 4-bit floats (17/64 of its bf16 bytes), which
 
 from __future__ import annotations
 
-import ctypes
 from typing import NamedTuple, Optional, Union
 
 import torch
@@ -18,9 +17,9 @@ import torch
 from . import _device as D
 from . import _lib
 
-
-def _blocks(hidden: int) -> int:
-    return -(-hidden // _lib.LPS_MX4_BLOCK)
+_pack_mx4 = _lib.packer(_lib.Mx4Args)
+_pack_embedding = _lib.packer(_lib.EmbeddingArgs)
+_pack_grad = _lib.packer(_lib.EmbeddingGradArgs)
 
 
 class Mx4Tensor(NamedTuple):
@@ -44,29 +43,36 @@ class Mx4Tensor(NamedTuple):
 
     def check(self, name: str) -> None:
         """Raises unless the parts are a 4-bit tensor on the GPU."""
-        D.require_device(self.codes, name + ".codes")
-        D.require_device(self.scales, name + ".scales")
-        if self.codes.dtype != torch.uint8 or self.scales.dtype != torch.uint8:
+        c, s, n = self.codes, self.scales, (self.hidden + 31) // 32
+        _on_gpu(c, name + ".codes")
+        _on_gpu(s, name + ".scales")
+        if c.dtype is not torch.uint8 or s.dtype is not torch.uint8:
             raise TypeError(f"{name}: codes and scales must be uint8")
-        n = _blocks(self.hidden)
-        if self.hidden < 1 or self.codes.dim() < 1 or self.codes.shape[-1] != 16 * n \
-                or self.scales.shape != (*self.codes.shape[:-1], n):
+        cs, ss = c.shape, s.shape
+        if n < 1 or len(cs) < 1 or len(ss) != len(cs) or cs[-1] != 16 * n or ss[-1] != n or cs[:-1] != ss[:-1]:
             raise ValueError(f"{name}: codes [..., {16 * n}] and scales [..., {n}] expected for rows of {self.hidden}; "
-                             f"got {tuple(self.codes.shape)}, {tuple(self.scales.shape)}")
-        if self.codes.device != self.scales.device:
-            raise ValueError(f"{name}: codes and scales are on different devices")
+                             f"got {tuple(cs)}, {tuple(ss)}")
+        _same_device(c, s, f"{name}: codes and scales")
 
     def rows(self):
         """(codes [R, 16 * blocks], scales [R, blocks]) with elements side by
         side and code rows on 16-byte lines."""
-        c, s = self.codes, self.scales
+        c, s, hidden = self
         if c.dim() != 2:
             c, s = c.reshape(-1, c.shape[-1]), s.reshape(-1, s.shape[-1])
-        if c.stride(1) != 1 or (c.shape[0] > 1 and (c.stride(0) % 16 or c.stride(0) < c.shape[1])) or c.data_ptr() % 16:
+        many, n = c.shape[0] > 1, c.shape[1]
+        r, e = c.stride()
+        if e != 1 or (many and (r % 16 or r < n)) or c.data_ptr() % 16:
             c = c.clone(memory_format=torch.contiguous_format)
-        if (s.stride(1) != 1 and s.shape[1] > 1) or (s.shape[0] > 1 and s.stride(0) < s.shape[1]):
+        r, e = s.stride()
+        if (e != 1 and n > 16) or (many and r < n // 16):
             s = s.contiguous()
         return c, s
+
+
+def _on_gpu(t: torch.Tensor, name: str) -> None:
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        D.require_device(t, name)
 
 
 def _flat_rows(x: torch.Tensor) -> torch.Tensor:
@@ -74,14 +80,23 @@ def _flat_rows(x: torch.Tensor) -> torch.Tensor:
     broadcast gradient's are not)."""
     if x.dim() != 2:
         x = x.reshape(-1, x.shape[-1])
-    if (x.stride(1) != 1 and x.shape[1] > 1) or (x.stride(0) < x.shape[1] and x.shape[0] > 1):
+    r, e = x.stride()
+    n, h = x.shape
+    if (e != 1 and h > 1) or (r < h and n > 1):
         x = x.contiguous()
     return x
 
 
 def _same_device(a: torch.Tensor, b: torch.Tensor, what: str) -> None:
-    if a.device != b.device:
+    if a.get_device() != b.get_device():
         raise ValueError(f"{what} are on different devices: {a.device}, {b.device}")
+
+
+def _call(name: str, args: bytes, device: torch.device) -> None:
+    with D.guard(device):
+        rc = getattr(_lib.load(), name)(args, D.stream_of(device))
+    if rc:
+        _lib.check(rc, name)
 
 
 def mx4_quantize(x: torch.Tensor) -> Mx4Tensor:
@@ -93,24 +108,27 @@ def mx4_quantize(x: torch.Tensor) -> Mx4Tensor:
     4, 6 to ``|x| / 2^s`` (ties to the even code, 6 above it; signs are kept).  A
     block with a value that is not finite becomes NaN.  ``H`` need not be a
     multiple of 32."""
-    D.require_device(x, "x")
-    code = D.dtype_code(x)
+    _on_gpu(x, "x")
+    code = D.code_of(x.dtype)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"x [..., H] with H >= 1 expected; got {tuple(x.shape)}")
-    lead, hidden = x.shape[:-1], x.shape[-1]
     xf = _flat_rows(x)
-    n, rows = _blocks(hidden), xf.shape[0]
-    codes = torch.empty((rows, 16 * n), dtype=torch.uint8, device=x.device)
+    device = x.device
+    rows, hidden = xf.shape
+    n = (hidden + 31) // 32
+    codes = torch.empty((rows, 16 * n), dtype=torch.uint8, device=device)
     # scale rows on 4-byte lines: the LM head reads four at a time
-    scales = torch.empty((rows, n + -n % 4), dtype=torch.uint8, device=x.device)[:, :n]
+    scales = torch.empty((rows, n + -n % 4), dtype=torch.uint8, device=device)
+    if n % 4:
+        scales = scales[:, :n]
     if rows:
-        a = _lib.Mx4Args(xf.data_ptr(), codes.data_ptr(), scales.data_ptr(), code, rows, hidden,
-                         xf.stride(0) if rows > 1 else hidden, codes.stride(0), scales.stride(0))
-        with D.guard(x.device):
-            rc = _lib.load().lps_mx4_quantize(ctypes.byref(a), D.stream_of(x.device))
-        _lib.check(rc, "lps_mx4_quantize")
-    if len(lead) != 1:
-        codes, scales = codes.view(*lead, 16 * n), scales.unflatten(0, lead) if lead else scales[0]
+        _call("lps_mx4_quantize",
+              _pack_mx4(xf.data_ptr(), codes.data_ptr(), scales.data_ptr(), code, rows, hidden,
+                        xf.stride(0) if rows > 1 else hidden, 16 * n, n + -n % 4), device)
+    if xf is not x:
+        lead = x.shape[:-1]
+        if len(lead) != 1:
+            codes, scales = codes.view(*lead, 16 * n), scales.unflatten(0, lead) if lead else scales[0]
     return Mx4Tensor(codes, scales, hidden)
 
 
@@ -118,61 +136,56 @@ def mx4_dequantize(t: Mx4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.T
     """The values ``[..., H]`` of a 4-bit tensor, in ``dtype`` (every one is
     exact in bfloat16 and float32)."""
     t.check("t")
+    code = D.code_of(dtype)
     codes, scales = t.rows()
-    rows = codes.shape[0]
-    out = torch.empty((rows, t.hidden), dtype=dtype, device=codes.device)
-    code = D.dtype_code(out)
+    rows, device, hidden = codes.shape[0], codes.device, t.hidden
+    out = torch.empty((rows, hidden), dtype=dtype, device=device)
     if rows:
-        a = _lib.Mx4Args(out.data_ptr(), codes.data_ptr(), scales.data_ptr(), code, rows, t.hidden, t.hidden,
-                         codes.stride(0) if rows > 1 else codes.shape[1], scales.stride(0) if rows > 1 else scales.shape[1])
-        with D.guard(codes.device):
-            rc = _lib.load().lps_mx4_dequantize(ctypes.byref(a), D.stream_of(codes.device))
-        _lib.check(rc, "lps_mx4_dequantize")
-    return out.reshape(t.shape)
+        many = rows > 1
+        _call("lps_mx4_dequantize",
+              _pack_mx4(out.data_ptr(), codes.data_ptr(), scales.data_ptr(), code, rows, hidden, hidden,
+                        codes.stride(0) if many else codes.shape[1], scales.stride(0) if many else scales.shape[1]), device)
+    return out if t.codes.dim() == 2 else out.reshape(t.shape)
 
 
 def _ids(ids: torch.Tensor) -> torch.Tensor:
-    D.require_device(ids, "ids")
-    if ids.dtype not in (torch.int64, torch.int32):
+    """ids as a vector of neighbouring elements."""
+    _on_gpu(ids, "ids")
+    if ids.dtype is not torch.int64 and ids.dtype is not torch.int32:
         raise TypeError(f"ids must be int64 or int32; got {ids.dtype}")
-    return ids.reshape(-1).contiguous()
+    return ids if ids.dim() == 1 and ids.is_contiguous() else ids.reshape(-1).contiguous()
 
 
 def _embedding(ids: torch.Tensor, table: Union[torch.Tensor, Mx4Tensor], scale: float,
                out_dtype: Optional[torch.dtype]) -> torch.Tensor:
     flat = _ids(ids)
-    a = _lib.EmbeddingArgs()
     if isinstance(table, Mx4Tensor):
         table.check("table")
         if table.codes.dim() != 2:
             raise ValueError(f"table [V, H] expected; got {tuple(table.shape)}")
         rows, scales = table.rows()
-        hidden = table.hidden
-        a.dtype, a.scales = _lib.LPS_DTYPE_MX4, scales.data_ptr()
-        a.scales_stride = scales.stride(0) if rows.shape[0] > 1 else scales.shape[1]
+        hidden, code, dtype = table.hidden, _lib.LPS_DTYPE_MX4, out_dtype or torch.bfloat16
+        vocab = rows.shape[0]
+        sp, ss = scales.data_ptr(), scales.stride(0) if vocab > 1 else scales.shape[1]
     else:
-        D.require_device(table, "table")
+        _on_gpu(table, "table")
+        code, dtype = D.code_of(table.dtype), out_dtype or table.dtype
         if table.dim() != 2 or table.shape[1] < 1:
             raise ValueError(f"table [V, H] expected; got {tuple(table.shape)}")
-        a.dtype = D.dtype_code(table)
-        rows, hidden = _flat_rows(table), table.shape[1]
+        rows = _flat_rows(table)
+        vocab, hidden = rows.shape
+        sp = ss = 0
     _same_device(ids, rows, "ids and table")
-    if rows.shape[0] < 1:
+    if vocab < 1:
         raise ValueError("the table has no rows")
-    out = torch.empty((flat.shape[0], hidden), device=rows.device,
-                      dtype=out_dtype or (torch.bfloat16 if isinstance(table, Mx4Tensor) else table.dtype))
-    a.out_dtype = D.dtype_code(out)
-    if flat.shape[0]:
-        a.ids, a.table, a.out = flat.data_ptr(), rows.data_ptr(), out.data_ptr()
-        a.id_bytes = flat.element_size()
-        a.n, a.vocab, a.hidden = flat.shape[0], rows.shape[0], hidden
-        a.table_stride = rows.stride(0) if rows.shape[0] > 1 else rows.shape[1]
-        a.out_stride = hidden
-        a.scale = scale
-        with D.guard(rows.device):
-            rc = _lib.load().lps_embedding(ctypes.byref(a), D.stream_of(rows.device))
-        _lib.check(rc, "lps_embedding")
-    return out.reshape(*ids.shape, hidden)
+    device, n = rows.device, flat.shape[0]
+    out_code = D.code_of(dtype)
+    out = torch.empty((n, hidden), device=device, dtype=dtype)
+    if n:
+        _call("lps_embedding",
+              _pack_embedding(flat.data_ptr(), rows.data_ptr(), sp, out.data_ptr(), flat.element_size(), code, out_code, n,
+                              vocab, hidden, rows.stride(0) if vocab > 1 else rows.shape[1], ss, hidden, scale), device)
+    return out if flat is ids else out.reshape(*ids.shape, hidden)
 
 
 class _Embedding(torch.autograd.Function):
@@ -214,40 +227,35 @@ def embedding_grad(ids: torch.Tensor, grad: torch.Tensor, vocab: int, scale: flo
     left alone) and ``out`` returned.  The order of the sum depends on ids and
     sizes alone: equal calls give equal bits."""
     flat = _ids(ids)
-    D.require_device(grad, "grad")
-    code = D.dtype_code(grad)
+    _on_gpu(grad, "grad")
+    code = D.code_of(grad.dtype)
     if grad.dim() != ids.dim() + 1 or grad.shape[:-1] != ids.shape or grad.shape[-1] < 1:
         raise ValueError(f"ids [...] and grad [..., H] expected; got {tuple(ids.shape)}, {tuple(grad.shape)}")
     if vocab < 1:
         raise ValueError(f"vocab must be at least 1; got {vocab}")
     _same_device(ids, grad, "ids and grad")
-    hidden, n = grad.shape[-1], flat.shape[0]
+    device, hidden, n = grad.device, grad.shape[-1], flat.shape[0]
     g = _flat_rows(grad)
     if out is None:
-        res = torch.empty((vocab, hidden), dtype=dtype or grad.dtype, device=grad.device)
+        dtype = dtype or grad.dtype
+        out_code = D.code_of(dtype)
+        res = torch.empty((vocab, hidden), dtype=dtype, device=device)
     else:
-        D.require_device(out, "out")
+        _on_gpu(out, "out")
         _same_device(out, grad, "out and grad")
         if dtype is not None and dtype != out.dtype:
             raise TypeError(f"dtype {dtype} and out of {out.dtype}")
-        if tuple(out.shape) != (vocab, hidden) or (hidden > 1 and out.stride(1) != 1) or (vocab > 1 and out.stride(0) < hidden):
+        out_code = D.code_of(out.dtype)
+        if out.shape != (vocab, hidden) or (hidden > 1 and out.stride(1) != 1) or (vocab > 1 and out.stride(0) < hidden):
             raise ValueError(f"out [{vocab}, {hidden}] with rows of neighbouring elements expected; got "
                              f"{tuple(out.shape)}, strides {out.stride()}")
         if out.requires_grad and torch.is_grad_enabled():
             raise ValueError("out requires a gradient; pass its .grad, or a detached tensor")
         res = out
-    lib = _lib.load()
-    need = lib.lps_embedding_grad_workspace_bytes(n, vocab, hidden)
-    ws = torch.empty((need,), dtype=torch.uint8, device=grad.device)
-    a = _lib.EmbeddingGradArgs()
-    a.ids, a.grad, a.out = flat.data_ptr(), g.data_ptr(), res.data_ptr()
-    a.id_bytes, a.dtype, a.out_dtype = flat.element_size(), code, D.dtype_code(res)
-    a.n, a.vocab, a.hidden = n, vocab, hidden
-    a.grad_stride = g.stride(0) if n > 1 else hidden
-    a.out_stride = res.stride(0) if vocab > 1 else hidden
-    a.scale, a.accumulate = scale, int(out is not None)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), need
-    with D.guard(grad.device):
-        rc = lib.lps_embedding_grad(ctypes.byref(a), D.stream_of(grad.device))
-    _lib.check(rc, "lps_embedding_grad")
+    need = _lib.load().lps_embedding_grad_workspace_bytes(n, vocab, hidden)
+    ws = torch.empty((need,), dtype=torch.uint8, device=device)
+    _call("lps_embedding_grad",
+          _pack_grad(flat.data_ptr(), g.data_ptr(), res.data_ptr(), flat.element_size(), code, out_code, n, vocab, hidden,
+                     g.stride(0) if n > 1 else hidden, res.stride(0) if vocab > 1 else hidden, scale,
+                     0 if out is None else 1, ws.data_ptr(), need), device)
     return res

@@ -82,3 +82,4 @@ inline C mfma_fp4(A a, A b, C c, int sa, int isa, int sb, int isb) {
   ([&] { const ::lps_emu::h2v t_ = (p); return ::lps_emu::put_pair((o), (double)t_.x, (double)t_.y, (s), (sel)); }())
 #define __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, fa, fb, sa, isa, sb, isb) \
   (::lps_emu::mfma_fp4((a), (b), (c), (sa), (isa), (sb), (isb)))
+#define __builtin_amdgcn_sched_barrier(mask) ((void)0)
