@@ -33,46 +33,64 @@ struct Mx4HeadParams {
   int wide;                  // rows of scales lie and end on 16-byte lines
 };
 
-// One workgroup of WM x WN waves computes a BM x BN tile; K is walked in stages of
-// NB blocks (32 NB values) through a ring of NS LDS buffers, filled by loads that
-// cost no registers (lps_lmhead.h).  A stage holds the x rows, then the w rows (16
-// bytes a block, chunk c of row r at place c ^ f(r)).  XB: bytes of a block of x,
-// 64 or 16.  A row has 4 bytes of scales where it has 64 of codes: loaded by the
-// stage they cost as many cache lines as the codes do (2048 x 4096 -> 151936 in 4
-// bits 1112 us, 732 without them), so that they come 32 blocks at a time, into two
-// buffers of their own.
+// One workgroup of WM x WN x KW waves computes a BM x BN tile; the KW groups of waves
+// take turns at K, two blocks at a time, and add their accumulators at the end.  x
+// and w stream into LDS rings of their own by loads that cost no registers
+// (lps_lmhead.h): w in NSW stages of 8 blocks, x in NSX stages of XNB.  The first
+// NXW waves load x, the others w and the scales: a wave's loads land in their
+// order, so that one which loads both could not wait for x (soon there, from the
+// caches) without waiting for the w stages ahead of it.
+// - Rows of w are read in whole lines of 128 bytes (8 blocks): reads of 64 bytes
+//   reach 3.5 TB/s of HBM here, of 128 bytes 7.0 (28 and 55 bytes a clock and CU
+//   out of the L2), of 16 bytes 0.9.
+// - Scales, a byte to 16 of codes, come 32 blocks at a time into two buffers: read
+//   by the stage they cost more than a third of the time (2048 x 4096 -> 151936 in
+//   4 bits 1112 us, 732 without them).
+// A stage's row r keeps its 16-byte chunk c at place c ^ f(r).  Of x, XR rows are
+// held (row r stands in for r + XR, ..: results that are dropped).  XB: bytes of a
+// block of x, 64 or 16.
+constexpr int M4_NB = 8;
 constexpr int M4_SB = 32;
+constexpr int M4_PER = M4_SB / M4_NB;
 constexpr int64_t M4_MAX_STRIDE = 1 << 23;   // bytes: 256 rows of it fit 32-bit offsets
-template <int BM_, int BN_, int WM_, int WN_, int NB_, int NS_, int WPE_, int XB_>
+template <int BM_, int BN_, int WM_, int WN_, int KW_, int XNB_, int NSX_, int NSW_, int NXW_, int WPE_, int XB_, int XR_ = BM_>
 struct M4Tile {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NB = NB_, NS = NS_, WPE = WPE_, XB = XB_;
-  static constexpr int NW = WM * WN, NT = 64 * NW;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, KW = KW_, XNB = XNB_, NSX = NSX_, NSW = NSW_;
+  static constexpr int NXW = NXW_, WPE = WPE_, XB = XB_, XR = XR_;
+  static constexpr int EW = WM * WN;                            // waves of one group (the epilogue's)
+  static constexpr int NWK = EW * KW, NTK = 64 * NWK, NWW = NWK - NXW;
   static constexpr int MT = BM / WM / 32, CT = BN / WN / 32;    // accumulators per wave: rows x columns
   static constexpr int WTN = 32 * CT;
-  static constexpr int XC = NB * XB / 16, WC = NB;              // 16-byte chunks per row
+  static constexpr int XC = XNB * XB / 16, WC = M4_NB;          // 16-byte chunks per row
   static constexpr int XRI = 64 / XC, WRI = 64 / WC;            // rows a wave's load instruction covers
-  static constexpr int XI = BM / XRI, WI = BN / WRI;            // load instructions of a stage
-  static constexpr int XPW = (XI + NW - 1) / NW, WPW = WI / NW; // ... of a wave (with more waves than XI some load the same)
+  static constexpr int XI = XR / XRI, WI = BN / WRI;            // load instructions of a stage
+  static constexpr int XPW = (XI + NXW - 1) / NXW, WPW = WI / NWW;   // ... of a wave (with more waves than XI some load the same)
   static constexpr bool XS = XB == 16;
-  static constexpr int SROWS = BN + (XS ? BM : 0);              // rows with scales: w's, then x's
-  static constexpr int LPW = XPW + WPW;
-  static constexpr int XBYTES = BM * XC * 16, WBYTES = BN * WC * 16;
-  static constexpr int STAGE = XBYTES + WBYTES;
-  static constexpr int SBYTES = SROWS * M4_SB;
-  static constexpr int KS = NB / 2;                             // steps of two blocks
-  static constexpr int PER = M4_SB / NB;                        // stages to a buffer of scales
-  static_assert(NB == 4 || NB == 8, "chunk places");
-  static_assert((XI % NW == 0 || NW % XI == 0) && WI % NW == 0, "whole load instructions per wave");
-  static_assert(BN % 32 == 0 && BM % 32 == 0, "whole loads of scales");
-  static_assert(BM % (32 * WM) == 0 && BN % (32 * WN) == 0 && BN % LMH_BN == 0, "tile shape");
-  static_assert(PER >= NS - 1, "scales are asked for before the stage that needs them");
-  static_assert((NS - 1) * LPW + 4 * SROWS / 32 / NW + 1 < 64, "the load counter holds 63");
+  static constexpr int SROWS = BN + (XS ? XR : 0);              // rows with scales: w's, then x's
+  static constexpr int XBYTES = XR * XC * 16, WBYTES = BN * WC * 16, SBYTES = SROWS * M4_SB;
+  static constexpr int WOFF = NSX * XBYTES, SOFF = WOFF + NSW * WBYTES, BYTES = SOFF + 2 * SBYTES;
+  static constexpr int ITS = M4_NB / XNB;                       // x stages to one of w
+  static constexpr int JS = XNB / 2 / KW;                       // pairs of blocks of a wave per x stage
+  static_assert(XNB == 4 || XNB == 8, "x stages");
+  static_assert(NXW * XRI % 8 == 0 || XPW == 1, "the rows of a lane's loads share their permutation");
+  static_assert((XI % NXW == 0 || NXW % XI == 0) && WI % NWW == 0 && NXW < NWK, "whole load instructions per wave");
+  static_assert(SROWS % 32 == 0 && XR % 8 == 0 && BM % XR == 0, "whole loads of scales");
+  static_assert(BM % (32 * WM) == 0 && BN % (32 * WN) == 0 && BN % LMH_BN == 0 && JS >= 1, "tile shape");
+  static_assert(M4_PER >= NSW - 1, "scales are asked for before the stage that needs them");
+  static_assert((NSW - 1) * WPW + SROWS / 8 / NWW + 1 < 64 && (NSX - 1) * XPW < 64, "the load counter holds 63");
   __device__ __forceinline__ static int xperm(int row) { return XC >= 8 ? (row & 7) : ((row >> 1) & 3); }
-  __device__ __forceinline__ static int wperm(int row) { return WC >= 8 ? (row & 7) : ((row >> 1) & 3); }
+  __device__ __forceinline__ static int wperm(int row) { return row & 7; }
+};
+// The waves that write a tile out, as lmh_epilogue sees them.
+template <typename T>
+struct M4Epi {
+  static constexpr int BM = T::BM, BN = T::BN, WM = T::WM, WN = T::WN, MT = T::MT, CT = T::CT, WTN = T::WTN;
+  static constexpr int NW = T::EW, NT = 64 * T::EW;
 };
 template <typename T, int ES>
 constexpr int m4_lds_bytes() {
-  return T::NS * T::STAGE + 2 * T::SBYTES > lmh_epi_bytes<T, ES>() ? T::NS * T::STAGE + 2 * T::SBYTES : lmh_epi_bytes<T, ES>();
+  constexpr int epi = lmh_epi_bytes<M4Epi<T>, ES>();
+  return T::BYTES > epi ? T::BYTES : epi;
 }
 
 #ifndef LPS_HOST_EMU
@@ -80,16 +98,21 @@ constexpr int m4_lds_bytes() {
 __device__ __forceinline__ uint32_t m4_lds(const char* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
 }
-// 16 / 4 bytes per lane from base + off (base uniform) to LDS at (uniform) dst + 16 / 4 * lane.
+// 16 / 4 bytes per lane from base + off (base uniform) to LDS at (uniform) dst + 16 /
+// 4 * lane.  The compiler does not see a load here: five wait states stand between
+// it and a vector instruction that may have written base just before (a reload of
+// a spilled scalar register).
 template <bool NTL>
 __device__ __forceinline__ void m4_dma16(const char* base, uint32_t off, uint32_t dst) {
+  dst = (uint32_t)__builtin_amdgcn_readfirstlane((int)dst);
   if constexpr (NTL)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(dst), "v"(off), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(dst), "v"(off), "s"(base) : "memory", "m0");
   else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(off), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(off), "s"(base) : "memory", "m0");
 }
 __device__ __forceinline__ void m4_dma4(const char* base, uint32_t off, uint32_t dst) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(dst), "v"(off), "s"(base) : "memory");
+  dst = (uint32_t)__builtin_amdgcn_readfirstlane((int)dst);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, %2" ::"s"(dst), "v"(off), "s"(base) : "memory", "m0");
 }
 #else
 inline uint64_t m4_lds(const char* p) { return (uint64_t)(uintptr_t)p; }
@@ -101,6 +124,26 @@ inline void m4_dma4(const char* base, uint32_t off, uint64_t dst) {
   memcpy(reinterpret_cast<char*>(dst) + 4 * ((int)threadIdx.x & 63), base + off, 4);
 }
 #endif
+#ifndef LPS_HOST_EMU
+template <int N>
+__device__ __forceinline__ void m4_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void m4_barrier() {   // this wave's LDS reads are done, then every wave's
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+#else
+template <int N>
+inline void m4_wait() {}
+inline void m4_barrier() { __syncthreads(); }
+#endif
+// Until at most `left` stages of PW loads each are in flight (left <= MAX).
+template <int PW, int MAX>
+__device__ __forceinline__ void m4_wait_left(int left) {
+  if constexpr (MAX == 0) m4_wait<0>();
+  else if (left >= MAX) m4_wait<MAX * PW>();
+  else m4_wait_left<PW, MAX - 1>(left);
+}
 
 // Eight codes as one fragment of the 16-bit instruction.
 template <int DT>
@@ -148,31 +191,37 @@ __device__ __forceinline__ bool m4_far_scale(uint32_t w) {
   return far;
 }
 
-// The position of a lane in a tile, and its reads of a stage.
+// The position of a lane in a tile, and its reads of the stages.  A stage's chunks
+// of w are those of its 8 blocks; scales point at the first block of the x stage.
 template <typename T>
 struct M4Lane {
-  int half, xr, wr, px, pw;
-  __device__ __forceinline__ M4Lane(int wm, int wn, int l)
-      : half(l >> 5), xr(wm * (T::MT * 32) + (l & 31)), wr(wn * T::WTN + (l & 31)), px(T::xperm(xr)), pw(T::wperm(wr)) {}
-  // (rows 32 apart share their permutation)
-  __device__ __forceinline__ u32x4 x(const char* stage, int i, int c) const {
-    return *reinterpret_cast<const u32x4*>(stage + ((xr + 32 * i) * T::XC + (c ^ px)) * 16);
+  int half, kg, xr, wr, px, pw;
+  __device__ __forceinline__ M4Lane(int wv, int l) {
+    const int e = wv % T::EW;
+    half = l >> 5;
+    kg = wv / T::EW;
+    xr = (e / T::WN) * (T::MT * 32) + (l & 31);
+    wr = (e % T::WN) * T::WTN + (l & 31);
+    px = T::xperm(xr % T::XR);      // (rows 32 apart share their permutation)
+    pw = T::wperm(wr);
   }
-  __device__ __forceinline__ u32x4 w(const char* stage, int i, int c) const {
-    return *reinterpret_cast<const u32x4*>(stage + T::XBYTES + ((wr + 32 * i) * T::WC + (c ^ pw)) * 16);
+  __device__ __forceinline__ u32x4 x(const char* xs, int i, int c) const {
+    return *reinterpret_cast<const u32x4*>(xs + ((xr + 32 * i) % T::XR * T::XC + (c ^ px)) * 16);
   }
-  // four blocks' scales of a row (word d of the stage); this lane's are in bytes 0 and 2
-  __device__ __forceinline__ uint32_t ws_all(const char* scales, int i, int d) const {
+  __device__ __forceinline__ u32x4 w(const char* ws, int i, int c) const {
+    return *reinterpret_cast<const u32x4*>(ws + ((wr + 32 * i) * T::WC + (c ^ pw)) * 16);
+  }
+  // four blocks' scales of a row
+  __device__ __forceinline__ uint32_t wscales(const char* scales, int i, int d) const {
     return *reinterpret_cast<const uint32_t*>(scales + (wr + 32 * i) * M4_SB + 4 * d);
   }
-  __device__ __forceinline__ uint32_t ws(const char* scales, int i, int d) const { return ws_all(scales, i, d) >> (8 * half); }
-  __device__ __forceinline__ uint32_t xs(const char* scales, int i, int d) const {
-    return *reinterpret_cast<const uint32_t*>(scales + (T::BN + xr + 32 * i) * M4_SB + 4 * d) >> (8 * half);
+  __device__ __forceinline__ uint32_t xscales(const char* scales, int i, int d) const {
+    return *reinterpret_cast<const uint32_t*>(scales + (T::BN + (xr + 32 * i) % T::XR) * M4_SB + 4 * d);
   }
 };
 
-// A byte of a word of scales as the conversions' scale: its neighbours land in the
-// sign and the mantissa, which they ignore.
+// A byte of a word of scales (0, or with odd j 2) as the conversions' scale: its
+// neighbours land in the sign and the mantissa, which they ignore.
 __device__ __forceinline__ float m4_scale(uint32_t w, int j) { return __uint_as_float((j & 1) ? w << 7 : w << 23); }
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
@@ -183,22 +232,23 @@ __device__ __forceinline__ ACC m4_mma4(u32x4 a, u32x4 b, ACC c, uint32_t sa, uin
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(m4_operand(a), m4_operand(b), c, 4, 4, 0, (int)sa, 0, (int)sb);
 }
 
-// The accumulators plus `steps` steps of two blocks, one after another: the last
-// columns of a row, and (FAR) stages of fp16 with scales that it does not hold.
+// The accumulators plus the wave's share of `pairs` pairs of blocks, one after
+// another: the last columns of a row, and (FAR) stages of fp16 with scales that it
+// does not hold.  w0: the first pair's first block in the w stage.
 template <int XDT, typename T, bool FAR, typename ACC>
-__device__ __forceinline__ void m4_plain_stage(const char* stage, const char* scales, const M4Lane<T>& L,
-                                               ACC (&acc)[T::MT][T::CT], int steps) {
+__device__ __forceinline__ void m4_plain_stage(const char* xs, const char* ws, int w0, const char* scales, const M4Lane<T>& L,
+                                               ACC (&acc)[T::MT][T::CT], int pairs) {
 #pragma unroll 1
-  for (int j = 0; j < steps; j++) {
-    const int c = 2 * j + L.half;
+  for (int p = L.kg; p < pairs; p += T::KW) {
+    const int c = 2 * p + L.half;
 #pragma unroll
     for (int b = 0; b < T::CT; b++) {
-      const u32x4 cw = L.w(stage, b, c);
-      const uint32_t byte = (L.ws_all(scales, b, j >> 1) >> (8 * (c & 3))) & 255u;
+      const u32x4 cw = L.w(ws, b, w0 + c);
+      const uint32_t byte = (L.wscales(scales, b, c >> 2) >> (8 * (c & 3))) & 255u;
       if constexpr (T::XS) {
 #pragma unroll
         for (int a = 0; a < T::MT; a++)
-          acc[a][b] = m4_mma4(L.x(stage, a, c), cw, acc[a][b], L.xs(scales, a, j >> 1) >> (16 * (j & 1)), byte, 0);
+          acc[a][b] = m4_mma4(L.x(xs, a, c), cw, acc[a][b], L.xscales(scales, a, c >> 2) >> (8 * (c & 3)), byte, 0);
       } else {
         const float s = __uint_as_float(byte << 23);
 #pragma unroll
@@ -206,7 +256,7 @@ __device__ __forceinline__ void m4_plain_stage(const char* stage, const char* sc
           const u32x4 fw = m4_frag<FAR ? LPS_DTYPE_BF16 : XDT>(cw[q], s);
 #pragma unroll
           for (int a = 0; a < T::MT; a++) {
-            const u32x4 fx = L.x(stage, a, 4 * c + q);
+            const u32x4 fx = L.x(xs, a, 4 * c + q);
             if constexpr (FAR) {
               u32x4 hi, lo;
               m4_split(fx, hi, lo);
@@ -224,10 +274,10 @@ __device__ __forceinline__ void m4_plain_stage(const char* stage, const char* sc
 
 // XDT: BF16, F16 or MX4; T::XB 64 or 16 accordingly.
 template <int XDT, int ODT, typename T, bool NTL>
-__global__ __launch_bounds__(T::NT, T::WPE) void mx4head_kernel(Mx4HeadParams Q) {
+__global__ __launch_bounds__(T::NTK, T::WPE) void mx4head_kernel(Mx4HeadParams Q) {
   constexpr int ES = ODT == LPS_DTYPE_F32 ? 4 : 2;
   constexpr int ADT = XDT == LPS_DTYPE_F16 ? LPS_DTYPE_F16 : LPS_DTYPE_BF16;   // (the accumulators are alike)
-  constexpr int MT = T::MT, CT = T::CT, NB = T::NB, KS = T::KS;
+  constexpr int MT = T::MT, CT = T::CT, NB = M4_NB, XNB = T::XNB, KW = T::KW, JS = T::JS;
   __shared__ __attribute__((aligned(1024))) char lds[m4_lds_bytes<T, ES>()];
   const LmHeadParams& P = Q.h;
   // tiles over the XCDs as in lmhead_kernel: a run each, the row tiles of one column tile first
@@ -236,7 +286,8 @@ __global__ __launch_bounds__(T::NT, T::WPE) void mx4head_kernel(Mx4HeadParams Q)
   if (((int)blockIdx.x >> 3) >= per || t >= P.tiles) return;   // uniform over the workgroup
   const int m0 = (t % P.mtiles) * T::BM, n0 = (t / P.mtiles) * T::BN;
   const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), l = (int)threadIdx.x & 63;
-  const int wm = wv / T::WN, wn = wv % T::WN;
+  const bool loads_x = wv < T::NXW;
+  const int lw = loads_x ? wv : wv - T::NXW;                   // among the waves that load the same
   const int64_t xstep = T::XS ? P.x_stride : 2 * P.x_stride;   // bytes of a row of x
   const char* const X = reinterpret_cast<const char*>(P.x) + (int64_t)m0 * xstep;
   const char* const W = reinterpret_cast<const char*>(P.w) + (int64_t)n0 * P.w_stride;
@@ -245,137 +296,213 @@ __global__ __launch_bounds__(T::NT, T::WPE) void mx4head_kernel(Mx4HeadParams Q)
   auto mrow = [&](int r) { return m0 + r < P.M ? r : P.M - 1 - m0; };
   auto nrow = [&](int r) { return n0 + r < P.V ? r : P.V - 1 - n0; };
 
-  uint32_t xoff[T::XPW], woff[T::WPW];
+  // (128 accumulators, two sets of fragments and the loads' offsets do not fit a
+  // wave's 256 registers: there a step reads its own fragments, the other wave of
+  // the SIMD fills the gap, and offsets are computed when they are needed)
+  constexpr bool AHEAD = !(T::XS && MT * CT >= 8 && T::WPE > 1);
+  // offsets of this lane's chunk of the k-th row that its wave loads: rows k R + rl, R
+  // a multiple of 8 (so that the place in the row is the same), clamped to the last
+  const int rl = loads_x ? lw % T::XI * T::XRI + l / T::XC : lw * T::WRI + l / T::WC;
+  const uint32_t rstep = loads_x ? (uint32_t)xstep : (uint32_t)P.w_stride;
+  const uint32_t rnext = rstep * (uint32_t)(loads_x ? T::NXW * T::XRI : T::NWW * T::WRI);
+  const uint32_t rlast = (uint32_t)(loads_x ? mrow(T::XR - 1) : nrow(T::BN - 1)) * rstep;
+  const uint32_t roff = (uint32_t)rl * rstep;
+  const uint32_t coff = (uint32_t)(loads_x ? (l % T::XC) ^ T::xperm(rl) : (l % T::WC) ^ T::wperm(rl)) * 16u;
+  constexpr int LPM = T::XPW > T::WPW ? T::XPW : T::WPW;
+  uint32_t offs[AHEAD ? LPM : 1];
+  if constexpr (AHEAD) {
 #pragma unroll
-  for (int i = 0; i < T::XPW; i++) {
-    const int row = ((i * T::NW + wv) % T::XI) * T::XRI + l / T::XC, c = (l % T::XC) ^ T::xperm(row);
-    xoff[i] = (uint32_t)mrow(row) * (uint32_t)xstep + c * 16;
+    for (int k = 0; k < LPM; k++) {
+      const uint32_t o = roff + (uint32_t)k * rnext;
+      offs[k] = (o < rlast ? o : rlast) + coff;
+    }
   }
-#pragma unroll
-  for (int i = 0; i < T::WPW; i++) {
-    const int row = (i * T::NW + wv) * T::WRI + l / T::WC, c = (l % T::WC) ^ T::wperm(row);
-    woff[i] = (uint32_t)nrow(row) * (uint32_t)P.w_stride + c * 16;
-  }
-  const auto lds0 = m4_lds(lds);
-  auto issue = [&](int s, int buf) {   // stage s into ring buffer buf
-    const char* xb = X + (int64_t)s * (NB * T::XB);
-    const char* wb = W + (int64_t)s * (NB * 16);
-    const auto d = lds0 + buf * T::STAGE;
-#pragma unroll
-    for (int i = 0; i < T::XPW; i++) m4_dma16<false>(xb, xoff[i], d + ((i * T::NW + wv) % T::XI) * 1024);
-#pragma unroll
-    for (int i = 0; i < T::WPW; i++) m4_dma16<NTL>(wb, woff[i], d + T::XBYTES + (i * T::NW + wv) * 1024);
+  auto off = [&](int k) {
+    if constexpr (AHEAD) return offs[k];
+    uint32_t o = roff;
+    LPS_KEEP_VGPR(o);
+    o += (uint32_t)k * rnext;
+    return (o < rlast ? o : rlast) + coff;
   };
-  const int ns = P.H / (32 * NB);   // whole stages of whole blocks; the rest of H follows them
+  const auto lds0 = m4_lds(lds);
+  auto issue_x = [&](int i, int slot) {
+    const char* base = X + (int64_t)i * (XNB * T::XB);
+#pragma unroll
+    for (int k = 0; k < T::XPW; k++)
+      m4_dma16<false>(base, off(k), lds0 + slot * T::XBYTES + ((k * T::NXW + lw) % T::XI) * 1024);
+  };
+  auto issue_w = [&](int s, int slot) {
+    const char* base = W + (int64_t)s * (NB * 16);
+#pragma unroll
+    for (int k = 0; k < T::WPW; k++)
+      m4_dma16<NTL>(base, off(k), lds0 + T::WOFF + slot * T::WBYTES + (k * T::NWW + lw) * 1024);
+  };
+  const int ns = P.H / (32 * NB), its = ns * T::ITS;   // whole stages of whole blocks; the rest of H follows them
   // scales of blocks 32 u .. +31, as far as the whole stages go: a row's 32 bytes
   // by two lanes, or by eight where it does not lie on 16-byte lines
-  char* const sbuf = lds + T::NS * T::STAGE;
-  const auto sdst = lds0 + T::NS * T::STAGE;
   const char* const WS = reinterpret_cast<const char*>(Q.ws) + (int64_t)n0 * Q.ws_stride;
   const char* const XSC = T::XS ? reinterpret_cast<const char*>(Q.xs) + (int64_t)m0 * Q.xs_stride : nullptr;
   auto issue_scales = [&](int u) {
-    const auto d = sdst + (u & 1) * T::SBYTES;
+    const auto d = lds0 + T::SOFF + (u & 1) * T::SBYTES;
     const int rl = Q.wide ? 32 : 8, groups = T::SROWS / rl, r0 = Q.wide ? l >> 1 : l >> 3;
     int b = M4_SB * u + (Q.wide ? 16 * (l & 1) : 4 * (l & 7));
     b = b < NB * ns ? b : 0;          // (a row without them: others of its own)
-    for (int i = wv; i < groups; i += T::NW) {
+    for (int i = lw; i < groups; i += T::NWW) {
       const bool ofx = T::XS && rl * i >= T::BN;
       const char* base = ofx ? XSC : WS;
-      const uint32_t off = (ofx ? (uint32_t)mrow(rl * i + r0 - T::BN) * (uint32_t)Q.xs_stride
-                                : (uint32_t)nrow(rl * i + r0) * (uint32_t)Q.ws_stride) + b;
-      if (Q.wide) m4_dma16<false>(base, off, d + i * 1024);
-      else m4_dma4(base, off, d + i * 256);
+      const uint32_t o = (ofx ? (uint32_t)mrow(rl * i + r0 - T::BN) * (uint32_t)Q.xs_stride
+                              : (uint32_t)nrow(rl * i + r0) * (uint32_t)Q.ws_stride) + b;
+      if (Q.wide) m4_dma16<false>(base, o, d + i * 1024);
+      else m4_dma4(base, o, d + i * 256);
     }
   };
 
   typename MfmaOps<ADT>::acc acc[MT][CT] = {};
-  const M4Lane<T> L(wm, wn, l);
-  // Fragments are read one step ahead of their matrix instructions and, of a
+  const M4Lane<T> L(wv, l);
+  // Fragments are (AHEAD) read one step ahead of their matrix instructions and, of a
   // 16-bit x, the codes converted one ahead, in the shadow of the matrix cores;
   // the last step of a stage waits for the next one and reads its first.
-  constexpr int STEPS = T::XS ? KS : 4 * KS;       // matrix steps of a stage (64 or 16 values)
+  constexpr int STEPS = T::XS ? JS : 4 * JS;       // matrix steps of a wave in an x stage (64 or 16 values)
+  constexpr int WDS = (XNB + 3) / 4;               // words of scales of an x stage
   u32x4 fx[2][MT], cw[2][CT], fw[2][CT];
-  uint32_t sw[NB / 4][CT], sx[NB / 4][MT];
-  auto read_scales = [&](const char* scales) {
+  uint32_t sw[WDS][CT], sx[WDS][MT];
+  // pair jj of a wave is pair jj KW + kg of the stage: word and (after the shift)
+  // byte of its scales
+  auto word = [](int jj) { return KW == 2 ? jj : jj >> 1; };
+  auto odd = [](int jj) { return KW == 2 ? 0 : jj & 1; };
+  const int shift = 8 * L.half + (KW == 2 ? 16 * L.kg : 0);
+  auto read_word = [&](const char* scales, int d, int to) {
 #pragma unroll
-    for (int d = 0; d < NB / 4; d++) {
+    for (int i = 0; i < CT; i++) sw[to][i] = L.wscales(scales, i, d) >> shift;
+    if constexpr (T::XS) {
 #pragma unroll
-      for (int i = 0; i < CT; i++) sw[d][i] = L.ws(scales, i, d);
-      if constexpr (T::XS) {
-#pragma unroll
-        for (int i = 0; i < MT; i++) sx[d][i] = L.xs(scales, i, d);
-      }
+      for (int i = 0; i < MT; i++) sx[to][i] = L.xscales(scales, i, d) >> shift;
     }
   };
-  auto read_x = [&](const char* stage, int k) {    // for matrix step k
-    const int c = T::XS ? 2 * k + L.half : 4 * (2 * (k >> 2) + L.half) + (k & 3);
+  auto read_scales = [&](const char* scales) {
+    if constexpr (AHEAD) {
 #pragma unroll
-    for (int i = 0; i < MT; i++) fx[k & 1][i] = L.x(stage, i, c);
+      for (int d = 0; d < WDS; d++) read_word(scales, d, d);
+    }
   };
-  auto read_w = [&](const char* stage, int j) {    // for blocks 2 j and 2 j + 1
+  // (b: the buffer of registers)
+  auto read_x = [&](const char* xs, int k, int b) {   // for matrix step k
+    const int blk = 2 * ((T::XS ? k : k >> 2) * KW + L.kg) + L.half, c = T::XS ? blk : 4 * blk + (k & 3);
 #pragma unroll
-    for (int i = 0; i < CT; i++) cw[j & 1][i] = L.w(stage, i, 2 * j + L.half);
+    for (int i = 0; i < MT; i++) fx[b][i] = L.x(xs, i, c);
   };
-  auto convert = [&](int k) {
+  auto read_w = [&](const char* ws, int w0, int jj, int b) {   // for the wave's pair jj
+#pragma unroll
+    for (int i = 0; i < CT; i++) cw[b][i] = L.w(ws, i, w0 + 2 * (jj * KW + L.kg) + L.half);
+  };
+  auto convert = [&](int k, int b, int fb) {
     if constexpr (!T::XS) {
-      const int j = k >> 2;
+      const int jj = k >> 2;
 #pragma unroll
-      for (int i = 0; i < CT; i++) fw[k & 1][i] = m4_frag<XDT>(cw[j & 1][i][k & 3], m4_scale(sw[j >> 1][i], j));
+      for (int i = 0; i < CT; i++) fw[fb][i] = m4_frag<XDT>(cw[b][i][k & 3], m4_scale(sw[word(jj)][i], odd(jj)));
     }
   };
   auto far_scales = [&](const char* scales) {      // (uniform over the wave)
     bool far = false;
     if constexpr (XDT == LPS_DTYPE_F16) {
 #pragma unroll
-      for (int d = 0; d < NB / 4; d++)
+      for (int d = 0; d < WDS; d++)
 #pragma unroll
-        for (int i = 0; i < CT; i++) far = far || m4_far_scale(L.ws_all(scales, i, d));
+        for (int i = 0; i < CT; i++) far = far || m4_far_scale(L.wscales(scales, i, d));
       far = wballot(far) != 0;
     }
     return far;
   };
-  auto scales_of = [&](int s) { return sbuf + ((s / T::PER) & 1) * T::SBYTES + (s % T::PER) * NB; };
+  auto xslot = [&](int slot) { return lds + slot * T::XBYTES; };
+  auto wslot = [&](int slot) { return lds + T::WOFF + slot * T::WBYTES; };
+  auto scales_of = [&](int i) {                    // of x stage i
+    const int s = i / T::ITS;
+    return lds + T::SOFF + ((s / M4_PER) & 1) * T::SBYTES + (s % M4_PER) * NB + (i % T::ITS) * XNB;
+  };
   if (ns > 0) {
-    issue_scales(0);
-    for (int s = 0; s < T::NS && s < ns; s++) issue(s, s);
-    if (ns >= T::NS) lmh_wait_barrier<(T::NS - 1) * T::LPW>();
-    else lmh_wait_barrier<0>();
+    if (loads_x) {
+      for (int i = 0; i < T::NSX && i < its; i++) issue_x(i, i);
+      m4_wait_left<T::XPW, T::NSX - 1>(its - 1);
+    } else {
+      issue_scales(0);
+      for (int s = 0; s < T::NSW && s < ns; s++) issue_w(s, s);
+      m4_wait_left<T::WPW, T::NSW - 1>(ns - 1);
+    }
+    m4_barrier();
     read_scales(scales_of(0));
-    read_w(lds, 0);
-    read_x(lds, 0);
-    convert(0);
-    int buf = 0;
-    for (int s = 0; s < ns; s++) {
-      const char* cur = lds + buf * T::STAGE;
-      const int nb = buf + 1 == T::NS ? 0 : buf + 1;
-      const bool far = far_scales(scales_of(s));
-      if (XDT == LPS_DTYPE_F16 && far) m4_plain_stage<XDT, T, true>(cur, scales_of(s), L, acc, KS);
+    if constexpr (AHEAD) {
+      read_w(wslot(0), 0, 0, 0);
+      read_x(xslot(0), 0, 0);
+      convert(0, 0, 0);
+    }
+    int xb = 0, wb = 0;
+    // every wave holds its last fragments of stage i, stage i + 1 has landed (and its
+    // scales, asked for before it)
+    auto next_stage = [&](int i, int s, bool next_w) {
+      if (loads_x) m4_wait_left<T::XPW, T::NSX - 2>(its - 2 - i);
+      else if (next_w) m4_wait_left<T::WPW, T::NSW - 2>(ns - 2 - s);
+      m4_barrier();
+      if (loads_x) {
+        if (i + T::NSX < its) issue_x(i + T::NSX, xb);
+      } else if (next_w) {
+        if (s % M4_PER == 0 && s + M4_PER < ns) issue_scales(s / M4_PER + 1);
+        if (s + T::NSW < ns) issue_w(s + T::NSW, wb);
+      }
+      read_scales(scales_of(i + 1));
+    };
+    // (an odd number of pairs a stage: the buffers of registers swap from stage to stage)
+    auto stage = [&](int i, auto par_c) {
+      constexpr int PAR = decltype(par_c)::value;  // the buffer of the stage's first codes (4 bits: and fragments)
+      const int w0 = (i % T::ITS) * XNB, s = i / T::ITS;
+      const char* const xs = xslot(xb);
+      const char* const ws = wslot(wb);
+      const bool far = far_scales(scales_of(i));
+      if (XDT == LPS_DTYPE_F16 && far) m4_plain_stage<XDT, T, true>(xs, ws, w0, scales_of(i), L, acc, XNB / 2);
+      const int nxb = xb + 1 == T::NSX ? 0 : xb + 1;
+      const bool next_w = (i + 1) % T::ITS == 0;
+      const int nwb = !next_w ? wb : wb + 1 == T::NSW ? 0 : wb + 1;
 #pragma unroll
       for (int k = 0; k < STEPS; k++) {
-        if (k + 1 < STEPS) {
+        const int jj = T::XS ? k : k >> 2;
+        const int fb = T::XS ? (k + PAR) & 1 : k & 1, fn = fb ^ 1;             // fragments of this step, the next one's
+        const int cb = (jj + PAR) & 1, cn = cb ^ 1;                            // codes of this pair, the next one's
+        if constexpr (!AHEAD) {
+          read_w(ws, w0, k, 0);
+          read_x(xs, k, 0);
+          if (!odd(jj)) read_word(scales_of(i), word(jj), 0);
+#pragma unroll
+          for (int a = 0; a < MT; a++)
+#pragma unroll
+            for (int b = 0; b < CT; b++)
+              acc[a][b] = m4_mma4(fx[0][a], cw[0][b], acc[a][b], sx[0][a], sw[0][b], odd(jj));
+          if (k + 1 == STEPS && i + 1 < its) next_stage(i, s, next_w);
+        } else if (k + 1 < STEPS) {
           if (XDT == LPS_DTYPE_F16 && far) continue;
-          if constexpr (T::XS) read_w(cur, k + 1);
-          else if ((k & 3) == 1 && (k >> 2) + 1 < KS) read_w(cur, (k >> 2) + 1);
-          read_x(cur, k + 1);
+          if constexpr (T::XS) read_w(ws, w0, k + 1, cn);
+          else if ((k & 3) == 1 && jj + 1 < JS) read_w(ws, w0, jj + 1, cn);
+          read_x(xs, k + 1, fn);
           __builtin_amdgcn_sched_barrier(0);   // (the compiler would move the reads down to their use)
-        }
-        if (k + 1 == STEPS) {
-          uint32_t ow[CT], ox[MT];   // (this step's scales)
+#pragma unroll
+          for (int a = 0; a < MT; a++)
+#pragma unroll
+            for (int b = 0; b < CT; b++) {
+              if constexpr (T::XS) acc[a][b] = m4_mma4(fx[fb][a], cw[cb][b], acc[a][b], sx[word(jj)][a], sw[word(jj)][b], odd(jj));
+              else acc[a][b] = MfmaOps<ADT>::mma(fx[fb][a], fw[fb][b], acc[a][b]);
+            }
+          convert(k + 1, ((k + 1) >> 2) == jj ? cb : cn, fn);
+          __builtin_amdgcn_sched_barrier(0);
+        } else {
+          uint32_t ow[CT], ox[MT];             // (this step's scales)
           if constexpr (T::XS) {
 #pragma unroll
-            for (int i = 0; i < CT; i++) ow[i] = sw[NB / 4 - 1][i];
+            for (int b = 0; b < CT; b++) ow[b] = sw[word(jj)][b];
 #pragma unroll
-            for (int i = 0; i < MT; i++) ox[i] = sx[NB / 4 - 1][i];
+            for (int a = 0; a < MT; a++) ox[a] = sx[word(jj)][a];
           }
-          if (s + 1 < ns) {
-            // every wave holds its last fragments of stage s, stage s + 1 has landed
-            // (and its scales, asked for before it)
-            lmh_wait_stage<T>(ns - 2 - s);
-            if (s % T::PER == 0 && s + T::PER < ns) issue_scales(s / T::PER + 1);
-            if (s + T::NS < ns) issue(s + T::NS, buf);
-            read_scales(scales_of(s + 1));
-            read_w(lds + nb * T::STAGE, 0);
-            read_x(lds + nb * T::STAGE, 0);
+          if (i + 1 < its) {
+            next_stage(i, s, next_w);
+            read_w(wslot(nwb), ((i + 1) % T::ITS) * XNB, 0, cn);
+            read_x(xslot(nxb), 0, fn);
             __builtin_amdgcn_sched_barrier(0);
           }
           if (!(XDT == LPS_DTYPE_F16 && far)) {
@@ -383,48 +510,46 @@ __global__ __launch_bounds__(T::NT, T::WPE) void mx4head_kernel(Mx4HeadParams Q)
             for (int a = 0; a < MT; a++)
 #pragma unroll
               for (int b = 0; b < CT; b++) {
-                if constexpr (T::XS) acc[a][b] = m4_mma4(fx[k & 1][a], cw[k & 1][b], acc[a][b], ox[a], ow[b], k);
-                else acc[a][b] = MfmaOps<ADT>::mma(fx[k & 1][a], fw[k & 1][b], acc[a][b]);
+                if constexpr (T::XS) acc[a][b] = m4_mma4(fx[fb][a], cw[cb][b], acc[a][b], ox[a], ow[b], odd(jj));
+                else acc[a][b] = MfmaOps<ADT>::mma(fx[fb][a], fw[fb][b], acc[a][b]);
               }
           }
-          if (s + 1 < ns) convert(0);
-        } else {
-#pragma unroll
-          for (int a = 0; a < MT; a++)
-#pragma unroll
-            for (int b = 0; b < CT; b++) {
-              if constexpr (T::XS) acc[a][b] = m4_mma4(fx[k & 1][a], cw[k & 1][b], acc[a][b], sx[k >> 1][a], sw[k >> 1][b], k);
-              else acc[a][b] = MfmaOps<ADT>::mma(fx[k & 1][a], fw[k & 1][b], acc[a][b]);
-            }
-          convert(k + 1);
-          __builtin_amdgcn_sched_barrier(0);
+          if (i + 1 < its) convert(0, cn, fn);
         }
       }
-      buf = nb;
+      xb = nxb;
+      wb = nwb;
+    };
+    if constexpr (JS % 2 == 0 || !AHEAD) {
+      for (int i = 0; i < its; i++) stage(i, std::integral_constant<int, 0>{});
+    } else {
+      for (int i = 0; i < its; i += 2) {
+        stage(i, std::integral_constant<int, 0>{});
+        if (i + 1 < its) stage(i + 1, std::integral_constant<int, 1>{});
+      }
     }
-    __syncthreads();
+    m4_barrier();
   }
-  const int k0 = ns * 32 * NB;
-  if (k0 < P.H) {
-    // the columns past the last whole stage, zeros up to one (with scales of 1)
-    const int nblk = (P.H + 31) >> 5, b0 = ns * NB;
-    for (int i = threadIdx.x; i < T::BM * T::XC; i += T::NT) {
+  const int nblk = (P.H + 31) >> 5;
+  for (int b0 = ns * NB; b0 < nblk; b0 += XNB) {
+    // the columns past the last whole stage, zeros up to an x stage (with scales of 1)
+    for (int i = threadIdx.x; i < T::XR * T::XC; i += T::NTK) {
       const int row = i / T::XC, c = (i % T::XC) ^ T::xperm(row);
       u32x4 v = {0u, 0u, 0u, 0u};
       const char* xr = X + (int64_t)mrow(row) * xstep;
       if constexpr (T::XS) {
         if (b0 + c < nblk) v = *reinterpret_cast<const u32x4*>(xr + (b0 + c) * 16);
       } else {
-        const int e0 = k0 + 8 * c;
+        const int e0 = 32 * b0 + 8 * c;
         if (e0 < P.H) v = load_piece<ADT>(xr, e0, P.H).q[0];
       }
       *reinterpret_cast<u32x4*>(lds + i * 16) = v;
     }
-    char* wb = lds + T::XBYTES;
-    for (int i = threadIdx.x; i < T::BN * T::WC; i += T::NT) {
-      const int row = i / T::WC, b = b0 + ((i % T::WC) ^ T::wperm(row));
+    char* const wst = lds + T::WOFF;
+    for (int i = threadIdx.x; i < T::BN * T::WC; i += T::NTK) {
+      const int row = i / T::WC, c = (i % T::WC) ^ T::wperm(row), b = b0 + c;
       u32x4 v = {0u, 0u, 0u, 0u};
-      if (b < nblk) {
+      if (c < XNB && b < nblk) {
         v = *reinterpret_cast<const u32x4*>(W + (int64_t)nrow(row) * P.w_stride + b * 16);
 #pragma unroll
         for (int e = 0; e < 4; e++) {               // (codes past the row's end count as zeros, whatever they hold)
@@ -432,22 +557,51 @@ __global__ __launch_bounds__(T::NT, T::WPE) void mx4head_kernel(Mx4HeadParams Q)
           v[e] = keep >= 8 ? v[e] : keep <= 0 ? 0u : v[e] & ((1u << (4 * keep)) - 1u);
         }
       }
-      *reinterpret_cast<u32x4*>(wb + i * 16) = v;
+      *reinterpret_cast<u32x4*>(wst + i * 16) = v;
     }
-    for (int i = threadIdx.x; i < T::SROWS * NB; i += T::NT) {
-      const int row = i / NB, b = b0 + i % NB;
+    char* const sst = lds + T::SOFF;
+    for (int i = threadIdx.x; i < T::SROWS * XNB; i += T::NTK) {
+      const int row = i / XNB, b = b0 + i % XNB;
       const char* sr = WS + (int64_t)nrow(row < T::BN ? row : 0) * Q.ws_stride;
       if constexpr (T::XS)
         if (row >= T::BN) sr = XSC + (int64_t)mrow(row - T::BN) * Q.xs_stride;
-      sbuf[row * M4_SB + i % NB] = b < nblk ? sr[b] : (char)127;
+      sst[row * M4_SB + i % XNB] = b < nblk ? sr[b] : (char)127;
     }
     __syncthreads();
-    const int steps = (nblk - b0 + 1) / 2;
-    if (XDT == LPS_DTYPE_F16 && far_scales(sbuf)) m4_plain_stage<XDT, T, true>(lds, sbuf, L, acc, steps);
-    else m4_plain_stage<XDT, T, false>(lds, sbuf, L, acc, steps);
+    const int left = nblk - b0, pairs = ((left < XNB ? left : XNB) + 1) / 2;
+    if (XDT == LPS_DTYPE_F16 && far_scales(sst)) m4_plain_stage<XDT, T, true>(lds, wst, 0, sst, L, acc, pairs);
+    else m4_plain_stage<XDT, T, false>(lds, wst, 0, sst, L, acc, pairs);
     __syncthreads();
   }
-  lmh_epilogue<ADT, ODT, T>(P, lds, acc, n0, m0, wv, l);
+  if constexpr (KW == 2) {
+    // the second group's accumulators join the first's
+    static_assert(T::EW * MT * CT * 4096 <= T::BYTES, "they fit the stages' place");
+    u32x4* const d = reinterpret_cast<u32x4*>(lds) + (wv % T::EW) * (MT * CT * 256) + l;
+    if (L.kg == 1) {
+#pragma unroll
+      for (int a = 0; a < MT; a++)
+#pragma unroll
+        for (int b = 0; b < CT; b++)
+#pragma unroll
+          for (int q = 0; q < 4; q++)
+            d[((a * CT + b) * 4 + q) * 64] = u32x4{__float_as_uint(acc[a][b][4 * q]), __float_as_uint(acc[a][b][4 * q + 1]),
+                                                   __float_as_uint(acc[a][b][4 * q + 2]), __float_as_uint(acc[a][b][4 * q + 3])};
+    }
+    __syncthreads();
+    if (L.kg == 1) return;   // (later barriers count the waves that are left)
+#pragma unroll
+    for (int a = 0; a < MT; a++)
+#pragma unroll
+      for (int b = 0; b < CT; b++)
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          const u32x4 v = d[((a * CT + b) * 4 + q) * 64];
+#pragma unroll
+          for (int e = 0; e < 4; e++) acc[a][b][4 * q + e] = __fadd_rn(acc[a][b][4 * q + e], __uint_as_float(v[e]));
+        }
+    __syncthreads();
+  }
+  lmh_epilogue<ADT, ODT, M4Epi<T>>(P, lds, acc, n0, m0, wv, l);
 }
 
 }  // namespace lps

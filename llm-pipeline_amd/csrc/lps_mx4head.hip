@@ -13,21 +13,50 @@ template <int XDT, int ODT, typename T, bool NTL>
 hipError_t launch_mx4head(Mx4HeadParams Q, hipStream_t s) {
   Q.h.mtiles = (Q.h.M + T::BM - 1) / T::BM;
   Q.h.tiles = Q.h.mtiles * ((Q.h.V + T::BN - 1) / T::BN);
-  hipLaunchKernelGGL((mx4head_kernel<XDT, ODT, T, NTL>), dim3((unsigned)(Q.h.tiles + 7) / 8 * 8), dim3(T::NT), 0, s, Q);
+  hipLaunchKernelGGL((mx4head_kernel<XDT, ODT, T, NTL>), dim3((unsigned)(Q.h.tiles + 7) / 8 * 8), dim3(T::NTK), 0, s, Q);
   return hipGetLastError();
 }
-int mx4head_shape(int M) { return M <= 32 ? 0 : M <= 64 ? 1 : M <= 128 ? 2 : 3; }
+// The tile shape by rows and tiles.  A grid whose tiles all run at once takes the
+// smallest shape of which that is true: two workgroups of some shapes share a CU
+// (the third column).  Larger grids go by their rows: while w's pass over HBM is
+// the bound one row tile, so that it is read once and streamed past the caches.
+// Measured at hidden 4096 (us; x in 16 bits, by shape): 128 rows of V 8192 17, 23,
+// 46; 256 of 8192 25, 26, 48; 512 of 8192 47, 40, 60; 1024 of 8192 94, 78, 62; 128 of
+// 32000 45, 41, 50; 256 of 32000 85, 76, 58; 64 of 151936 -, 95, 160.  x in 4 bits:
+// 256 rows of V 8192 -, 13, 18, 35; 512 of 8192 -, 24, 21, 38; 1024 of 8192 -, 42, 29,
+// 40; 512 of 32000 -, 80, 49, 44; 512 of 151936 -, -, 258, 267; 2048 -, -, 956, 853.
+struct M4Shape { int bm, bn, per_cu, rows; };
+constexpr M4Shape M4_SHAPES16[] = {{32, 128, 2, 32}, {64, 128, 2, 64}, {128, 256, 1, 0}};
+constexpr M4Shape M4_SHAPES4[] = {{32, 128, 1, 32}, {64, 128, 1, 64}, {128, 128, 2, 256}, {256, 256, 1, 0}};
+template <int N>
+int mx4head_shape(const M4Shape (&shapes)[N], int M, int V, int cus) {
+  for (int i = 0; i < N; i++) {
+    const int64_t tiles = (int64_t)((M + shapes[i].bm - 1) / shapes[i].bm) * ((V + shapes[i].bn - 1) / shapes[i].bn);
+    if (tiles <= (int64_t)cus * shapes[i].per_cu || i + 1 == N || M <= shapes[i].rows) return i;
+  }
+  return N - 1;
+}
 
 template <int XDT, int ODT>
 hipError_t launch_mx4head_rows(const Mx4HeadParams& Q, hipStream_t s) {
-  constexpr int XB = XDT == DT_MX4 ? 16 : 64;
-  switch (mx4head_shape(Q.h.M)) {
-    case 0: return launch_mx4head<XDT, ODT, M4Tile<32, 128, 1, 4, 8, 3, 1, XB>, true>(Q, s);
-    case 1: return launch_mx4head<XDT, ODT, M4Tile<64, 128, 1, 4, 4, 4, 1, XB>, true>(Q, s);
-    case 2: return launch_mx4head<XDT, ODT, M4Tile<128, 128, 4, 2, 4, 3, 2, XB>, true>(Q, s);
-    default:
-      if constexpr (XB == 16) return launch_mx4head<XDT, ODT, M4Tile<256, 256, 4, 2, 4, 3, 2, XB>, false>(Q, s);
-      else return launch_mx4head<XDT, ODT, M4Tile<128, 256, 2, 2, 4, 2, 1, XB>, false>(Q, s);
+  const int M = Q.h.M, V = Q.h.V, cus = device_cus();
+  if constexpr (XDT == DT_MX4) {
+    switch (mx4head_shape(M4_SHAPES4, M, V, cus)) {
+      case 0: return launch_mx4head<XDT, ODT, M4Tile<32, 128, 1, 4, 2, 8, 2, 2, 4, 2, 16>, true>(Q, s);
+      case 1: return launch_mx4head<XDT, ODT, M4Tile<64, 128, 2, 2, 2, 8, 2, 2, 4, 2, 16>, true>(Q, s);
+      case 2: return launch_mx4head<XDT, ODT, M4Tile<128, 128, 2, 2, 1, 8, 2, 2, 2, 1, 16>, false>(Q, s);
+      default: return launch_mx4head<XDT, ODT, M4Tile<256, 256, 2, 4, 1, 8, 2, 2, 4, 2, 16>, false>(Q, s);
+    }
+  } else {
+    switch (mx4head_shape(M4_SHAPES16, M, V, cus)) {
+      case 0:
+        // few rows leave LDS for stages further ahead (8 rows of V 151936: 57 us, 74 with 32 held; 16: 63, 75)
+        if (M <= 8) return launch_mx4head<XDT, ODT, M4Tile<32, 128, 1, 4, 2, 8, 3, 3, 4, 2, 64, 8>, true>(Q, s);
+        if (M <= 16) return launch_mx4head<XDT, ODT, M4Tile<32, 128, 1, 4, 2, 8, 3, 3, 4, 2, 64, 16>, true>(Q, s);
+        return launch_mx4head<XDT, ODT, M4Tile<32, 128, 1, 4, 2, 4, 4, 2, 4, 2, 64>, true>(Q, s);
+      case 1: return launch_mx4head<XDT, ODT, M4Tile<64, 128, 2, 2, 2, 4, 2, 2, 4, 2, 64>, true>(Q, s);
+      default: return launch_mx4head<XDT, ODT, M4Tile<128, 256, 2, 4, 1, 4, 2, 2, 4, 2, 64>, false>(Q, s);
+    }
   }
 }
 template <int XDT>

@@ -78,10 +78,11 @@ _MX4_MAX_STRIDE = 1 << 23   # bytes between rows (include/lps.h)
 
 def _words(s: torch.Tensor) -> torch.Tensor:
     """Scales with rows on 4-byte lines, as the kernel reads them."""
-    if s.data_ptr() % 4 == 0 and (s.shape[0] <= 1 or s.stride(0) % 4 == 0):
+    rows, n = s.shape
+    r = s.stride(0) if rows > 1 else 0
+    if s.data_ptr() % 4 == 0 and r % 4 == 0 and r <= _MX4_MAX_STRIDE:
         return s
-    n = s.shape[1]
-    out = torch.empty((s.shape[0], n + -n % 4), dtype=torch.uint8, device=s.device)[:, :n]
+    out = torch.empty((rows, n + -n % 4), dtype=torch.uint8, device=s.device)[:, :n]
     return out.copy_(s)
 
 

@@ -9,6 +9,14 @@
 // its size.
 #include "mx4_ops.h"
 
+// The emulated device's compute units (LPS_EMU_CUS, 256 by default).
+inline hipError_t emu_cus(int* v) {
+  const char* e = getenv("LPS_EMU_CUS");
+  *v = e ? atoi(e) : 256;
+  return hipSuccess;
+}
+#define hipDeviceGetAttribute(v, attribute, device) emu_cus(v)
+
 #include "../../llm-pipeline_amd/csrc/lps_table.hip"
 #include "../../llm-pipeline_amd/csrc/lps_mx4head.hip"
 
