@@ -183,16 +183,15 @@ __device__ __forceinline__ void m4_split(u32x4 x, u32x4& hi, u32x4& lo) {
   }
 }
 
-// Whether any of four scale bytes is outside 104 .. 140 (2^-23 .. 2^13).
-__device__ __forceinline__ bool m4_far_scale(uint32_t w) {
-  bool far = false;
-#pragma unroll
-  for (int k = 0; k < 4; k++) far = far || ((w >> (8 * k)) & 255u) - 104u > 36u;
-  return far;
+// Nonzero when any of four scale bytes is outside 104 .. 140 (2^-23 .. 2^13): of a byte
+// under 128, 24 more must reach 128, of the low 7 bits of another 115 more must not.
+__device__ __forceinline__ uint32_t m4_far_scale(uint32_t w) {
+  const uint32_t low = (w & 0x7F7F7F7Fu) + 0x18181818u, high = (w & 0x7F7F7F7Fu) + 0x73737373u;
+  return ((~w & ~low) | (w & high)) & 0x80808080u;
 }
 
 // The position of a lane in a tile, and its reads of the stages.  A stage's chunks
-// of w are those of its 8 blocks; scales point at the first block of the x stage.
+// of w and its scales are those of its 8 blocks.
 template <typename T>
 struct M4Lane {
   int half, kg, xr, wr, px, pw;
@@ -244,11 +243,11 @@ __device__ __forceinline__ void m4_plain_stage(const char* xs, const char* ws, i
 #pragma unroll
     for (int b = 0; b < T::CT; b++) {
       const u32x4 cw = L.w(ws, b, w0 + c);
-      const uint32_t byte = (L.wscales(scales, b, c >> 2) >> (8 * (c & 3))) & 255u;
+      const uint32_t byte = (L.wscales(scales, b, (w0 + c) >> 2) >> (8 * ((w0 + c) & 3))) & 255u;
       if constexpr (T::XS) {
 #pragma unroll
         for (int a = 0; a < T::MT; a++)
-          acc[a][b] = m4_mma4(L.x(xs, a, c), cw, acc[a][b], L.xscales(scales, a, c >> 2) >> (8 * (c & 3)), byte, 0);
+          acc[a][b] = m4_mma4(L.x(xs, a, c), cw, acc[a][b], L.xscales(scales, a, (w0 + c) >> 2) >> (8 * ((w0 + c) & 3)), byte, 0);
       } else {
         const float s = __uint_as_float(byte << 23);
 #pragma unroll
@@ -363,7 +362,7 @@ __global__ __launch_bounds__(T::NTK, T::WPE) void mx4head_kernel(Mx4HeadParams Q
   // 16-bit x, the codes converted one ahead, in the shadow of the matrix cores;
   // the last step of a stage waits for the next one and reads its first.
   constexpr int STEPS = T::XS ? JS : 4 * JS;       // matrix steps of a wave in an x stage (64 or 16 values)
-  constexpr int WDS = (XNB + 3) / 4;               // words of scales of an x stage
+  constexpr int WDS = XNB / 4;               // words of scales of an x stage
   u32x4 fx[2][MT], cw[2][CT], fw[2][CT];
   uint32_t sw[WDS][CT], sx[WDS][MT];
   // pair jj of a wave is pair jj KW + kg of the stage: word and (after the shift)
@@ -371,18 +370,25 @@ __global__ __launch_bounds__(T::NTK, T::WPE) void mx4head_kernel(Mx4HeadParams Q
   auto word = [](int jj) { return KW == 2 ? jj : jj >> 1; };
   auto odd = [](int jj) { return KW == 2 ? 0 : jj & 1; };
   const int shift = 8 * L.half + (KW == 2 ? 16 * L.kg : 0);
-  auto read_word = [&](const char* scales, int d, int to) {
+  uint32_t far_any = 0;                            // fp16: whether this lane met a scale that it does not hold
+  auto read_word = [&](const char* scales, int w0, int d, int to) {
+    d += w0 >> 2;
 #pragma unroll
-    for (int i = 0; i < CT; i++) sw[to][i] = L.wscales(scales, i, d) >> shift;
+    for (int i = 0; i < CT; i++) {
+      const uint32_t w = L.wscales(scales, i, d);
+      if constexpr (XDT == LPS_DTYPE_F16) far_any |= m4_far_scale(w);
+      sw[to][i] = w >> shift;
+    }
     if constexpr (T::XS) {
 #pragma unroll
       for (int i = 0; i < MT; i++) sx[to][i] = L.xscales(scales, i, d) >> shift;
     }
   };
-  auto read_scales = [&](const char* scales) {
+  auto read_scales = [&](const char* scales, int w0) {
+    far_any = 0;
     if constexpr (AHEAD) {
 #pragma unroll
-      for (int d = 0; d < WDS; d++) read_word(scales, d, d);
+      for (int d = 0; d < WDS; d++) read_word(scales, w0, d, d);
     }
   };
   // (b: the buffer of registers)
@@ -402,23 +408,9 @@ __global__ __launch_bounds__(T::NTK, T::WPE) void mx4head_kernel(Mx4HeadParams Q
       for (int i = 0; i < CT; i++) fw[fb][i] = m4_frag<XDT>(cw[b][i][k & 3], m4_scale(sw[word(jj)][i], odd(jj)));
     }
   };
-  auto far_scales = [&](const char* scales) {      // (uniform over the wave)
-    bool far = false;
-    if constexpr (XDT == LPS_DTYPE_F16) {
-#pragma unroll
-      for (int d = 0; d < WDS; d++)
-#pragma unroll
-        for (int i = 0; i < CT; i++) far = far || m4_far_scale(L.wscales(scales, i, d));
-      far = wballot(far) != 0;
-    }
-    return far;
-  };
   auto xslot = [&](int slot) { return lds + slot * T::XBYTES; };
   auto wslot = [&](int slot) { return lds + T::WOFF + slot * T::WBYTES; };
-  auto scales_of = [&](int i) {                    // of x stage i
-    const int s = i / T::ITS;
-    return lds + T::SOFF + ((s / M4_PER) & 1) * T::SBYTES + (s % M4_PER) * NB + (i % T::ITS) * XNB;
-  };
+  auto scales_of = [&](int s) { return lds + T::SOFF + ((s / M4_PER) & 1) * T::SBYTES + (s % M4_PER) * NB; };
   if (ns > 0) {
     if (loads_x) {
       for (int i = 0; i < T::NSX && i < its; i++) issue_x(i, i);
@@ -429,7 +421,7 @@ __global__ __launch_bounds__(T::NTK, T::WPE) void mx4head_kernel(Mx4HeadParams Q
       m4_wait_left<T::WPW, T::NSW - 1>(ns - 1);
     }
     m4_barrier();
-    read_scales(scales_of(0));
+    read_scales(scales_of(0), 0);
     if constexpr (AHEAD) {
       read_w(wslot(0), 0, 0, 0);
       read_x(xslot(0), 0, 0);
@@ -448,7 +440,7 @@ __global__ __launch_bounds__(T::NTK, T::WPE) void mx4head_kernel(Mx4HeadParams Q
         if (s % M4_PER == 0 && s + M4_PER < ns) issue_scales(s / M4_PER + 1);
         if (s + T::NSW < ns) issue_w(s + T::NSW, wb);
       }
-      read_scales(scales_of(i + 1));
+      read_scales(scales_of((i + 1) / T::ITS), (i + 1) % T::ITS * XNB);
     };
     // (an odd number of pairs a stage: the buffers of registers swap from stage to stage)
     auto stage = [&](int i, auto par_c) {
@@ -456,8 +448,8 @@ __global__ __launch_bounds__(T::NTK, T::WPE) void mx4head_kernel(Mx4HeadParams Q
       const int w0 = (i % T::ITS) * XNB, s = i / T::ITS;
       const char* const xs = xslot(xb);
       const char* const ws = wslot(wb);
-      const bool far = far_scales(scales_of(i));
-      if (XDT == LPS_DTYPE_F16 && far) m4_plain_stage<XDT, T, true>(xs, ws, w0, scales_of(i), L, acc, XNB / 2);
+      const bool far = XDT == LPS_DTYPE_F16 && wballot(far_any != 0) != 0;   // (uniform over the wave)
+      if (XDT == LPS_DTYPE_F16 && far) m4_plain_stage<XDT, T, true>(xs, ws, w0, scales_of(s), L, acc, XNB / 2);
       const int nxb = xb + 1 == T::NSX ? 0 : xb + 1;
       const bool next_w = (i + 1) % T::ITS == 0;
       const int nwb = !next_w ? wb : wb + 1 == T::NSW ? 0 : wb + 1;
@@ -469,7 +461,7 @@ __global__ __launch_bounds__(T::NTK, T::WPE) void mx4head_kernel(Mx4HeadParams Q
         if constexpr (!AHEAD) {
           read_w(ws, w0, k, 0);
           read_x(xs, k, 0);
-          if (!odd(jj)) read_word(scales_of(i), word(jj), 0);
+          if (!odd(jj)) read_word(scales_of(s), w0, word(jj), 0);
 #pragma unroll
           for (int a = 0; a < MT; a++)
 #pragma unroll
@@ -569,7 +561,8 @@ __global__ __launch_bounds__(T::NTK, T::WPE) void mx4head_kernel(Mx4HeadParams Q
     }
     __syncthreads();
     const int left = nblk - b0, pairs = ((left < XNB ? left : XNB) + 1) / 2;
-    if (XDT == LPS_DTYPE_F16 && far_scales(sst)) m4_plain_stage<XDT, T, true>(lds, wst, 0, sst, L, acc, pairs);
+    if constexpr (XDT == LPS_DTYPE_F16) read_scales(sst, 0);
+    if (XDT == LPS_DTYPE_F16 && wballot(far_any != 0) != 0) m4_plain_stage<XDT, T, true>(lds, wst, 0, sst, L, acc, pairs);
     else m4_plain_stage<XDT, T, false>(lds, wst, 0, sst, L, acc, pairs);
     __syncthreads();
   }

@@ -48,13 +48,19 @@ hipError_t launch_mx4head_rows(const Mx4HeadParams& Q, hipStream_t s) {
       default: return launch_mx4head<XDT, ODT, M4Tile<256, 256, 2, 4, 1, 8, 2, 2, 4, 2, 16>, false>(Q, s);
     }
   } else {
+    // two workgroups to a CU: fp16's two paths have to be held to their 128 registers
+    // (bf16's fit by themselves; held to it, 16 rows take 74 us for 63)
+    constexpr int WPE = XDT == LPS_DTYPE_F16 ? 4 : 2;
     switch (mx4head_shape(M4_SHAPES16, M, V, cus)) {
       case 0:
         // few rows leave LDS for stages further ahead (8 rows of V 151936: 57 us, 74 with 32 held; 16: 63, 75)
-        if (M <= 8) return launch_mx4head<XDT, ODT, M4Tile<32, 128, 1, 4, 2, 8, 3, 3, 4, 2, 64, 8>, true>(Q, s);
-        if (M <= 16) return launch_mx4head<XDT, ODT, M4Tile<32, 128, 1, 4, 2, 8, 3, 3, 4, 2, 64, 16>, true>(Q, s);
-        return launch_mx4head<XDT, ODT, M4Tile<32, 128, 1, 4, 2, 4, 4, 2, 4, 2, 64>, true>(Q, s);
-      case 1: return launch_mx4head<XDT, ODT, M4Tile<64, 128, 2, 2, 2, 4, 2, 2, 4, 2, 64>, true>(Q, s);
+        if (M <= 8) return launch_mx4head<XDT, ODT, M4Tile<32, 128, 1, 4, 2, 8, 3, 3, 4, WPE, 64, 8>, true>(Q, s);
+        if (M <= 16) return launch_mx4head<XDT, ODT, M4Tile<32, 128, 1, 4, 2, 8, 3, 3, 4, WPE, 64, 16>, true>(Q, s);
+        return launch_mx4head<XDT, ODT, M4Tile<32, 128, 1, 4, 2, 4, 4, 2, 4, 4, 64>, true>(Q, s);
+      case 1:
+        // (fp16's second path does not fit 128 registers beside two columns of accumulators)
+        if constexpr (XDT == LPS_DTYPE_F16) return launch_mx4head<XDT, ODT, M4Tile<64, 128, 2, 4, 1, 4, 2, 2, 4, 4, 64>, true>(Q, s);
+        else return launch_mx4head<XDT, ODT, M4Tile<64, 128, 2, 2, 2, 4, 2, 2, 4, 4, 64>, true>(Q, s);
       default: return launch_mx4head<XDT, ODT, M4Tile<128, 256, 2, 4, 1, 4, 2, 2, 4, 2, 64>, false>(Q, s);
     }
   }
