@@ -3,6 +3,7 @@
 // (added to out[v] when accumulating), summed in fp32 in one fixed order, so a
 // call's result never depends on timing.
 //
+// Up to EG_SMALL positions, one launch: grad_small_kernel.  More, three:
 // 1. grad_sort_kernel groups the positions by id.  Workgroup w of G takes the
 //    ids with id % G == w (neighbouring frequent ids land apart); it reads all
 //    ids, counts its own and those of the workgroups before it (its place in
@@ -24,10 +25,12 @@ namespace lps {
 
 constexpr int EG_NT = 1024;         // threads of the sort
 constexpr int EG_NW = EG_NT / 64;
-constexpr int EG_HIST = 16384;      // ids a workgroup of the sort can own
+constexpr int EG_OWN = 1024;        // ids a workgroup of the sort can own
 constexpr int EG_LIST = 4096;       // positions it keeps in LDS
 constexpr int EG_SMAX = 256;        // positions of a tile, at most
-constexpr int EG_FILL_ROWS = 16;    // rows a zeroing workgroup looks at
+constexpr int EG_FILL = 8192;       // bytes of rows that a zeroing workgroup looks at, or one row
+constexpr int EG_JOIN = 8;          // tiles a joining workgroup looks at
+constexpr int EG_SMALL = 2048;      // positions of the one-launch form
 
 struct EmbGradParams {
   const void* ids;
@@ -39,6 +42,7 @@ struct EmbGradParams {
   int accumulate;
   int lg_groups;         // log2 G
   int S, tiles, slices;  // positions of a tile; tiles; workgroups on a tile
+  int fill_rows;         // rows of a zeroing workgroup
   // workspace
   int* count;            // [1] positions with a valid id
   int* sid;              // [n] ids in the order
@@ -50,112 +54,141 @@ struct EmbGradParams {
   int64_t part_stride;
 };
 
+// What bounds the sort is latency: every workgroup reads all ids (from its L2), lists
+// its own in order (waves take runs of positions), and cuts the list into a run per
+// wave: counts by id and wave, one scan over both, and each wave places its run.
+// 8192 ids 13 us, 32768 19 us (with one wave that places the whole list 17 and 27).
 __global__ __launch_bounds__(EG_NT) void grad_sort_kernel(EmbGradParams P) {
-  __shared__ uint32_t hist[EG_HIST];
+  __shared__ uint32_t count[EG_NW][EG_OWN];        // positions of an id in a wave's run; then their next place
   __shared__ int list_id[EG_LIST], list_pos[EG_LIST];
   __shared__ int wcnt[EG_NW], wless[EG_NW], wall[EG_NW];
   __shared__ uint32_t wsum[EG_NW];
   const int tid = (int)threadIdx.x, wv = tid >> 6, l = tid & 63;
   const int w = (int)blockIdx.x, lg = P.lg_groups, mask = (1 << lg) - 1;
   const int own = w < P.vocab ? (P.vocab - 1 - w) / (mask + 1) + 1 : 0;   // ids w, w + G, ..
-  for (int k = tid; k < own; k += EG_NT) hist[k] = 0;
-  __syncthreads();
-  // each wave takes a run of positions, 64 at a time
+  // each wave takes a run of positions, 64 U at a time
   const int per = ((P.n + EG_NW - 1) / EG_NW + 63) & ~63;
   const int64_t a64 = (int64_t)wv * per;
   const int a = a64 < P.n ? (int)a64 : P.n, b = P.n - a < per ? P.n : a + per;
-  constexpr int U = 8;
-  int cnt = 0, less = 0, all = 0;
-  for (int i0 = a; i0 < b; i0 += 64 * U) {
-    int64_t id[U];
+  constexpr int U = 8, R = 4;                      // (R batches are kept for the second pass)
+  int kept[R][U];                                  // ids (-1 without one)
+  auto fetch = [&](int i0, int (&id)[U]) {
+    int64_t v[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
       const int64_t i = (int64_t)i0 + 64 * u + l;
-      id[u] = i < b ? load_id(P.ids, P.id_bytes, i) : -1;
+      v[u] = i < b ? load_id(P.ids, P.id_bytes, i) : -1;
     }
 #pragma unroll
+    for (int u = 0; u < U; u++) id[u] = v[u] >= 0 && v[u] < P.vocab ? (int)v[u] : -1;
+  };
+#pragma unroll
+  for (int r = 0; r < R; r++)
+    if ((int64_t)a + 64 * U * r < b) fetch(a + 64 * U * r, kept[r]);
+  for (int k = l; k < own; k += 64) count[wv][k] = 0;
+  int cnt = 0, less = 0, all = 0;                  // this lane's
+  auto tally = [&](const int (&id)[U]) {
+#pragma unroll
     for (int u = 0; u < U; u++) {
-      const bool valid = id[u] >= 0 && id[u] < P.vocab;
-      const int g = (int)id[u] & mask;
-      const bool mine = valid && g == w;
-      cnt += __builtin_popcountll(wballot(mine));
-      less += __builtin_popcountll(wballot(valid && g < w));
-      all += __builtin_popcountll(wballot(valid));
-      if (mine) atomicAdd(&hist[(int)id[u] >> lg], 1u);
+      const bool valid = id[u] >= 0;
+      cnt += valid && (id[u] & mask) == w;
+      less += valid && (id[u] & mask) < w;
+      all += valid;
     }
+  };
+#pragma unroll
+  for (int r = 0; r < R; r++)
+    if ((int64_t)a + 64 * U * r < b) tally(kept[r]);
+  for (int64_t i0 = (int64_t)a + 64 * U * R; i0 < b; i0 += 64 * U) {
+    int id[U];
+    fetch((int)i0, id);
+    tally(id);
   }
+  cnt = lps::wsum(cnt);
+  less = lps::wsum(less);
+  all = lps::wsum(all);
   if (l == 0) { wcnt[wv] = cnt; wless[wv] = less; wall[wv] = all; }
   __syncthreads();
-  int start = 0, total = 0, mine0 = 0, every = 0;
+  int start = 0, total = 0, at = 0, every = 0;
   for (int k = 0; k < EG_NW; k++) {
     start += wless[k];
-    mine0 += k < wv ? wcnt[k] : 0;
+    at += k < wv ? wcnt[k] : 0;
     total += wcnt[k];
     every += wall[k];
   }
   if (w == 0 && tid == 0) *P.count = every;
-  if (P.touched)
-    for (int k = tid; k < own; k += EG_NT) P.touched[w + ((int64_t)k << lg)] = hist[k] != 0;
-  if (total == 0) return;                          // (uniform over the workgroup)
-  // the ids' first places: an exclusive scan of the counts, a run of them per thread
-  {
-    const int run = (own + EG_NT - 1) / EG_NT, k0 = tid * run;
-    uint32_t s = 0;
-    for (int k = k0; k < k0 + run && k < own; k++) s += hist[k];
-    const uint32_t incl = wscan_incl(s);
-    if (l == 63) wsum[wv] = incl;
-    __syncthreads();
-    uint32_t at = incl - s;
-    for (int k = 0; k < wv; k++) at += wsum[k];
-    for (int k = k0; k < k0 + run && k < own; k++) {
-      const uint32_t c = hist[k];
-      hist[k] = at;
-      at += c;
-    }
-  }
   // the workgroup's positions in their own order
   const bool in_lds = total <= EG_LIST;
   int* const gid = P.tmp_id + start;
   int* const gpos = P.tmp_pos + start;
-  int at = mine0;
-  for (int i0 = a; i0 < b; i0 += 64 * U) {
-    int64_t id[U];
+  auto place = [&](int i0, const int (&id)[U]) {
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const int64_t i = (int64_t)i0 + 64 * u + l;
-      id[u] = i < b ? load_id(P.ids, P.id_bytes, i) : -1;
-    }
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-      const bool mine = id[u] >= 0 && id[u] < P.vocab && ((int)id[u] & mask) == w;
+      const bool mine = id[u] >= 0 && (id[u] & mask) == w;
       const uint64_t m = wballot(mine);
       if (mine) {
         const int k = at + (int)lanes_below(m), i = i0 + 64 * u + l;
-        if (in_lds) { list_id[k] = (int)id[u] >> lg; list_pos[k] = i; }
-        else { gid[k] = (int)id[u] >> lg; gpos[k] = i; }
+        if (in_lds) { list_id[k] = id[u] >> lg; list_pos[k] = i; }
+        else { gid[k] = id[u] >> lg; gpos[k] = i; }
       }
       at += __builtin_popcountll(m);
     }
+  };
+#pragma unroll
+  for (int r = 0; r < R; r++)
+    if ((int64_t)a + 64 * U * r < b) place(a + 64 * U * r, kept[r]);
+  for (int64_t i0 = (int64_t)a + 64 * U * R; i0 < b; i0 += 64 * U) {
+    int id[U];
+    fetch((int)i0, id);
+    place((int)i0, id);
   }
   __syncthreads();
-  if (wv != 0) return;
-  // 64 at a time: a position's place is its id's next one, after the lower
-  // lanes of the same id (found bit by bit of the id)
-  const int bits = 32 - __builtin_clz((uint32_t)own);
-  for (int k0 = 0; k0 < total; k0 += 64) {
-    const int k = k0 + l;
-    const bool on = k < total;
-    const int id = on ? (in_lds ? list_id[k] : gid[k]) : 0;
-    const int pos = on ? (in_lds ? list_pos[k] : gpos[k]) : 0;
+  // this wave's run of the list
+  const int run = ((total + EG_NW - 1) / EG_NW + 63) & ~63;
+  const int k0 = wv * run < total ? wv * run : total, k1 = total - k0 < run ? total : k0 + run;
+  for (int k = k0 + l; k < k1; k += 64) atomicAdd(&count[wv][in_lds ? list_id[k] : gid[k]], 1u);
+  __syncthreads();
+  {
+    // a thread's id: its positions over the waves, its place over the ids
+    uint32_t c[EG_NW], s = 0;
+    if (tid < own) {
+#pragma unroll
+      for (int k = 0; k < EG_NW; k++) {
+        c[k] = count[k][tid];
+        s += c[k];
+      }
+    }
+    if (P.touched && tid < own) P.touched[w + ((int64_t)tid << lg)] = s != 0;
+    const uint32_t incl = wscan_incl(s);
+    if (l == 63) wsum[wv] = incl;
+    __syncthreads();
+    uint32_t p = incl - s;
+    for (int k = 0; k < wv; k++) p += wsum[k];
+    if (tid < own) {
+#pragma unroll
+      for (int k = 0; k < EG_NW; k++) {
+        count[k][tid] = p;
+        p += c[k];
+      }
+    }
+  }
+  __syncthreads();
+  // 64 positions at a time: a position's place is its id's next one in this run, after
+  // the lower lanes of the same id (found bit by bit of the id)
+  const int bits = 32 - __builtin_clz((uint32_t)own | 1u);
+  for (int q = k0; q < k1; q += 64) {
+    const int k = q + l;
+    const bool on = k < k1;
+    const int id = on ? (in_lds ? list_id[k] : gid[k]) : 0, pos = on ? (in_lds ? list_pos[k] : gpos[k]) : 0;
     uint64_t same = wballot(on);
-    for (int q = 0; q < bits; q++) {
-      const bool one = (id >> q) & 1;
+    for (int i = 0; i < bits; i++) {
+      const bool one = (id >> i) & 1;
       const uint64_t m = wballot(one);
       same &= one ? m : ~m;
     }
     const int rank = (int)lanes_below(same), first = same ? __builtin_ctzll(same) : l;
     uint32_t base = 0;
-    if (on && rank == 0) base = atomicAdd(&hist[id], (uint32_t)__builtin_popcountll(same));
+    if (on && rank == 0) base = atomicAdd(&count[wv][id], (uint32_t)__builtin_popcountll(same));
     base = (uint32_t)__shfl((int)base, first, 64);
     if (on) {
       P.sid[start + (int)base + rank] = (id << lg) + w;
@@ -186,14 +219,16 @@ __global__ __launch_bounds__(256) void grad_tiles_kernel(EmbGradParams P) {
   const int tid = (int)threadIdx.x;
   const int64_t work = (int64_t)P.tiles * P.slices;
   if (blockIdx.x >= work) {
-    // rows without a token
-    const int64_t r0 = ((int64_t)blockIdx.x - work) * EG_FILL_ROWS;
+    // rows without a token: as many neighbouring ones as EG_FILL bytes hold, so that
+    // the launch writes memory in its order (1.2 GB in rows of 8 KB: 194 us at a row
+    // to a workgroup, 215 at 16, 231 at 149)
+    const int64_t r0 = ((int64_t)blockIdx.x - work) * P.fill_rows;
     const float zero[8] = {};
-    for (int r = 0; r < EG_FILL_ROWS; r++) {
-      const int64_t row = r0 + r;
-      if (row >= P.vocab || P.touched[row]) continue;
-      char* o = static_cast<char*>(P.out) + row * P.out_stride * ElemBytes<ODT>::value;
-      for (int e0 = 8 * tid; e0 < P.hidden; e0 += 8 * 256) store_piece<ODT>(o, e0, P.hidden, zero);
+    const int pieces = (P.hidden + 7) >> 3;
+    for (int i = tid; i < P.fill_rows * pieces; i += 256) {
+      const int64_t row = r0 + i / pieces;
+      if (row < P.vocab && !P.touched[row])
+        store_piece<ODT>(static_cast<char*>(P.out) + row * P.out_stride * ElemBytes<ODT>::value, 8 * (i % pieces), P.hidden, zero);
     }
     return;
   }
@@ -256,38 +291,13 @@ __global__ __launch_bounds__(256) void grad_tiles_kernel(EmbGradParams P) {
   flush(cur, m);
 }
 
-// One workgroup per tile and 256 columns: 32 threads of eight columns, eight of
-// them on every eighth partial row, added in order at the end.
-template <int ODT>
-__global__ __launch_bounds__(256) void grad_join_kernel(EmbGradParams P) {
-  __shared__ float red[8][256 + 8];
-  const int t = (int)blockIdx.x, nv = *P.count;
-  const int64_t end = ((int64_t)t + 1) * P.S;
-  if (end >= nv) return;                           // the order's last tile: no run leaves it
-  const int id = P.sid[end - 1];
-  if (P.sid[end] != id) return;
-  const int64_t base = end - P.S;
-  if (base > 0 && P.sid[base] == id && P.sid[base - 1] == id) return;   // the run began in an earlier tile
-  const int c = (int)threadIdx.x & 31, k = (int)threadIdx.x >> 5;
-  const int e0 = 256 * (int)blockIdx.y + 8 * c;
-  float acc[8] = {};
-  if (e0 < P.hidden) {
-    auto add = [&](int64_t row) {
-      const u32x4* p = reinterpret_cast<const u32x4*>(P.part + row * P.part_stride + e0);
-      const u32x4 x = p[0], y = p[1];
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        acc[e] = __fadd_rn(acc[e], __uint_as_float(x[e]));
-        acc[4 + e] = __fadd_rn(acc[4 + e], __uint_as_float(y[e]));
-      }
-    };
-    if (k == 0) add(2 * (int64_t)t + 1);
-    for (int64_t q = (int64_t)t + 1 + k; q * P.S < nv && P.sid[q * P.S] == id; q += 8) add(2 * q);
-  }
+// Columns e0 .. e0 + 7 of the eight threads that share them added in order: true in
+// the first of the eight, with the sum in acc.
+__device__ __forceinline__ bool grad_reduce8(float (&red)[8][256 + 8], int c, int k, float (&acc)[8]) {
 #pragma unroll
   for (int e = 0; e < 8; e++) red[k][8 * c + e] = acc[e];
   __syncthreads();
-  if (k == 0 && e0 < P.hidden) {
+  if (k == 0) {
 #pragma unroll
     for (int e = 0; e < 8; e++) {
       float s = acc[e];
@@ -295,7 +305,179 @@ __global__ __launch_bounds__(256) void grad_join_kernel(EmbGradParams P) {
       for (int q = 1; q < 8; q++) s = __fadd_rn(s, red[q][8 * c + e]);
       acc[e] = s;
     }
-    grad_write<ODT>(P, id, e0, acc);
+  }
+  __syncthreads();
+  return k == 0;
+}
+
+// One workgroup per EG_JOIN tiles and 256 columns, 32 threads of eight columns to a
+// tile: they add the partial rows of the run that begins in it and leaves it, or,
+// where it goes through more than EG_LONG tiles, all 256 do, every eighth row each
+// and those eight sums in order.
+constexpr int EG_LONG = 16;
+template <int ODT>
+__global__ __launch_bounds__(256) void grad_join_kernel(EmbGradParams P) {
+  static_assert(EG_JOIN == 8, "a group of threads to a tile");
+  __shared__ float red[8][256 + 8];
+  __shared__ int s_id[EG_JOIN], s_tiles[EG_JOIN];
+  const int nv = *P.count;
+  const int c = (int)threadIdx.x & 31, k = (int)threadIdx.x >> 5;
+  const int e0 = 256 * (int)blockIdx.y + 8 * c;
+  auto add = [&](int64_t row, float (&acc)[8]) {
+    const u32x4* p = reinterpret_cast<const u32x4*>(P.part + row * P.part_stride + e0);
+    const u32x4 x = p[0], y = p[1];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      acc[e] = __fadd_rn(acc[e], __uint_as_float(x[e]));
+      acc[4 + e] = __fadd_rn(acc[4 + e], __uint_as_float(y[e]));
+    }
+  };
+  const int64_t t0 = (int64_t)blockIdx.x * EG_JOIN;
+  {
+    // tile t0 + k: not the order's last one, not one inside a run
+    const int64_t t = t0 + k, base = t * P.S, end = base + P.S;
+    int id = 0, tiles = 0;                         // (of the run: after this one)
+    bool open = false;
+    if (end < nv) {
+      id = P.sid[end - 1];
+      open = P.sid[end] == id && !(base > 0 && P.sid[base] == id && P.sid[base - 1] == id);
+    }
+    // the next tiles that begin with the id, 32 looked at at a time (two tiles a wave)
+    while (wballot(open)) {
+      const int64_t q = (t + 1 + tiles + c) * P.S;
+      const uint64_t all = wballot(open && q < nv && P.sid[q < nv ? q : 0] == id);
+      const uint32_t m = ~(uint32_t)(all >> (32 * (k & 1)));
+      if (open) tiles += m ? __builtin_ctz(m) : 32;
+      open = open && m == 0;
+    }
+    if (c == 0) {
+      s_id[k] = id;
+      s_tiles[k] = tiles;
+    }
+    if (tiles > 0 && tiles <= EG_LONG && e0 < P.hidden) {
+      float acc[8] = {};
+      add(2 * t + 1, acc);
+#pragma unroll 4
+      for (int q = 0; q < tiles; q++) add(2 * (t + 1 + q), acc);
+      grad_write<ODT>(P, id, e0, acc);
+    }
+  }
+  __syncthreads();
+  for (int j = 0; j < EG_JOIN; j++) {
+    const int tiles = s_tiles[j];
+    if (tiles <= EG_LONG) continue;                // (uniform over the workgroup)
+    const int64_t t = t0 + j;
+    float acc[8] = {};
+    if (e0 < P.hidden) {
+      if (k == 0) add(2 * t + 1, acc);
+#pragma unroll 4
+      for (int q = k; q < tiles; q += 8) add(2 * (t + 1 + q), acc);
+    }
+    if (grad_reduce8(red, c, k, acc) && e0 < P.hidden) grad_write<ODT>(P, s_id[j], e0, acc);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Few positions, one launch.  Workgroup (w, y) owns the ids with id % G == w and
+// 256 columns; it lists its positions in order and adds their rows: an id of few
+// positions by 32 threads (eight ids at a time), of more by all eight such
+// groups, every eighth listed position each.  Its other rows become zero.
+// ---------------------------------------------------------------------------
+template <int GDT, int ODT>
+__global__ __launch_bounds__(256) void grad_small_kernel(EmbGradParams P) {
+  __shared__ int first[EG_OWN];              // an id's first place in the list, and how often it is there
+  __shared__ uint32_t times[EG_OWN];
+  __shared__ unsigned short list_id[EG_SMALL], list_pos[EG_SMALL];
+  __shared__ int wcnt[4];
+  __shared__ float red[8][256 + 8];
+  const int tid = (int)threadIdx.x, wv = tid >> 6, l = tid & 63;
+  const int w = (int)blockIdx.x, lg = P.lg_groups, mask = (1 << lg) - 1;
+  const int own = w < P.vocab ? (P.vocab - 1 - w) / (mask + 1) + 1 : 0;
+  constexpr int U = EG_SMALL / 256;
+  const int per = EG_SMALL / 4, a = wv * per;      // this wave's positions, 64 at a time
+  int id[U], cnt = 0;
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    const int i = a + 64 * u + l;
+    const int64_t v = i < P.n ? load_id(P.ids, P.id_bytes, i) : -1;
+    id[u] = v >= 0 && v < P.vocab && ((int)v & mask) == w ? (int)v >> lg : -1;
+    cnt += __builtin_popcountll(wballot(id[u] >= 0));
+  }
+  for (int k = tid; k < own; k += 256) {
+    first[k] = EG_SMALL;
+    times[k] = 0;
+  }
+  if (l == 0) wcnt[wv] = cnt;
+  __syncthreads();
+  int at = 0, total = 0;
+  for (int k = 0; k < 4; k++) {
+    at += k < wv ? wcnt[k] : 0;
+    total += wcnt[k];
+  }
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    const uint64_t m = wballot(id[u] >= 0);
+    if (id[u] >= 0) {
+      const int k = at + (int)lanes_below(m);
+      list_id[k] = (unsigned short)id[u];
+      list_pos[k] = (unsigned short)(a + 64 * u + l);
+      atomicMin(&first[id[u]], k);
+      atomicAdd(&times[id[u]], 1u);
+    }
+    at += __builtin_popcountll(m);
+  }
+  __syncthreads();
+  const int c = tid & 31, k = tid >> 5;
+  const int e0 = 256 * (int)blockIdx.y + 8 * c;
+  const bool in = e0 < P.hidden;
+  constexpr uint32_t FEW = 16;
+  // the rows of list places j0, j0 + step, .. that hold the id
+  auto add = [&](int want, int j0, int step, float (&acc)[8]) {
+    constexpr int B = 4;
+    for (int j = j0; j < total; j += step * B) {
+      Piece<GDT> g[B];
+      bool on[B];
+#pragma unroll
+      for (int u = 0; u < B; u++) {
+        const int p = j + u * step;
+        on[u] = p < total && list_id[p] == want;
+        if (on[u])
+          g[u] = load_piece<GDT>(static_cast<const char*>(P.grad) + (int64_t)list_pos[p] * P.grad_stride * ElemBytes<GDT>::value,
+                                 e0, P.hidden);
+      }
+#pragma unroll
+      for (int u = 0; u < B; u++) {
+        if (on[u]) {
+          float v[8];
+          piece_values(g[u], v);
+#pragma unroll
+          for (int e = 0; e < 8; e++) acc[e] = __fadd_rn(acc[e], v[e]);
+        }
+      }
+    }
+  };
+  if (in) {
+    for (int j = k; j < total; j += 8) {
+      const int x = list_id[j];
+      if (first[x] != j || times[x] > FEW) continue;
+      float acc[8] = {};
+      add(x, j, 1, acc);
+      grad_write<ODT>(P, (x << lg) + w, e0, acc);
+    }
+    if (!P.accumulate) {
+      const float zero[8] = {};
+      for (int x = k; x < own; x += 8)
+        if (times[x] == 0)
+          store_piece<ODT, true>(static_cast<char*>(P.out) + (((int64_t)x << lg) + w) * P.out_stride * ElemBytes<ODT>::value,
+                                 e0, P.hidden, zero);
+    }
+  }
+  for (int j = 0; j < total; j++) {                // (uniform over the workgroup)
+    const int x = list_id[j];
+    if (first[x] != j || times[x] <= FEW) continue;
+    float acc[8] = {};
+    if (in) add(x, j + k, 8, acc);
+    if (grad_reduce8(red, c, k, acc) && in) grad_write<ODT>(P, (x << lg) + w, e0, acc);
   }
 }
 

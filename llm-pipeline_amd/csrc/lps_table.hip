@@ -63,10 +63,12 @@ struct EgWs {
 // Positions of a tile: about 2048 tiles, so that a frequent token's rows spread
 // over the card and a tile's loads are in flight together.
 int eg_tile(int n) {
-  int s = 4;
+  int s = 8;
   while (s < EG_SMAX && (int64_t)s * 2048 < n) s *= 2;
   return s;
 }
+// One launch, without a workspace: few positions, and ids that 4096 workgroups can own.
+bool eg_small(int n, int vocab) { return n <= EG_SMALL && vocab <= 4096 * EG_OWN; }
 EgWs eg_workspace(int n, int vocab, int hidden) {
   EgWs w{};
   size_t at = 0;
@@ -75,6 +77,7 @@ EgWs eg_workspace(int n, int vocab, int hidden) {
     at += (bytes + 255) / 256 * 256;
     return p;
   };
+  if (eg_small(n, vocab)) return w;
   const int S = eg_tile(n);
   const size_t tiles = ((size_t)n + S - 1) / S;
   w.count = take(4);
@@ -89,12 +92,23 @@ EgWs eg_workspace(int n, int vocab, int hidden) {
 }
 
 template <int GDT, int ODT>
-hipError_t launch_grad(const EmbGradParams& P, hipStream_t s) {
+hipError_t launch_grad(EmbGradParams P, hipStream_t s) {
+  if (eg_small(P.n, P.vocab)) {
+    // about eight positions and 64 thousand values of zeros a workgroup, up to one on
+    // each CU; more where it would own more ids than it can count
+    const int64_t values = P.accumulate ? 0 : (int64_t)P.vocab * (P.hidden < 256 ? P.hidden : 256);
+    int lg = 4;
+    while (lg < 8 && ((8 << lg) < P.n || (values >> lg) > 65536)) lg++;
+    while (((int64_t)P.vocab + (1 << lg) - 1) >> lg > EG_OWN) lg++;
+    P.lg_groups = lg;
+    hipLaunchKernelGGL((grad_small_kernel<GDT, ODT>), dim3(1u << lg, (unsigned)((P.hidden + 255) / 256)), dim3(256), 0, s, P);
+    return hipGetLastError();
+  }
   hipLaunchKernelGGL(grad_sort_kernel, dim3(1u << P.lg_groups), dim3(EG_NT), 0, s, P);
-  const int64_t fill = P.touched ? ((int64_t)P.vocab + EG_FILL_ROWS - 1) / EG_FILL_ROWS : 0;
+  const int64_t fill = P.touched ? ((int64_t)P.vocab + P.fill_rows - 1) / P.fill_rows : 0;
   hipLaunchKernelGGL((grad_tiles_kernel<GDT, ODT>), dim3((unsigned)((int64_t)P.tiles * P.slices + fill)), dim3(256), 0, s, P);
   if (P.tiles > 1)
-    hipLaunchKernelGGL((grad_join_kernel<ODT>), dim3((unsigned)(P.tiles - 1), (unsigned)((P.hidden + 255) / 256)), dim3(256), 0, s, P);
+    hipLaunchKernelGGL((grad_join_kernel<ODT>), dim3((unsigned)((P.tiles - 1 + EG_JOIN - 1) / EG_JOIN), (unsigned)((P.hidden + 255) / 256)), dim3(256), 0, s, P);
   return hipGetLastError();
 }
 template <int GDT>
@@ -205,8 +219,8 @@ int lps_embedding_grad(const lps_embedding_grad_args* a, void* stream) {
     return LPS_EINVAL;
   if ((a->n > 1 && a->grad_stride < a->hidden) || (a->vocab > 1 && a->out_stride < a->hidden)) return LPS_EINVAL;
   const EgWs w = eg_workspace(a->n, a->vocab, a->hidden);
-  if (!a->workspace || a->workspace_bytes < w.bytes) return LPS_EWORKSPACE;
-  if (!aligned_to(a->workspace, 16)) return LPS_EINVAL;
+  if (w.bytes && (!a->workspace || a->workspace_bytes < w.bytes)) return LPS_EWORKSPACE;
+  if (w.bytes && !aligned_to(a->workspace, 16)) return LPS_EINVAL;
   char* ws = static_cast<char*>(a->workspace);
   EmbGradParams P{};
   P.ids = a->ids;
@@ -220,16 +234,18 @@ int lps_embedding_grad(const lps_embedding_grad_args* a, void* stream) {
   P.id_bytes = a->id_bytes;
   P.scale = a->scale;
   P.accumulate = a->accumulate ? 1 : 0;
-  // workgroups of the sort: about 64 positions and at most 1024 ids each, up to
-  // one on each CU; more where a workgroup would own more ids than it can count
+  // workgroups of the sort: about 64 positions each, up to one on each CU; more where
+  // a workgroup would own more ids than it can count
   int lg = 3;
-  while (lg < 8 && (((int64_t)64 << lg) < a->n || (a->vocab >> lg) > 1024)) lg++;
-  while (((int64_t)a->vocab + (1 << lg) - 1) >> lg > EG_HIST) lg++;
+  while (lg < 8 && ((int64_t)64 << lg) < a->n) lg++;
+  while (((int64_t)a->vocab + ((int64_t)1 << lg) - 1) >> lg > EG_OWN) lg++;
   P.lg_groups = lg;
   P.S = eg_tile(a->n);
   P.tiles = (int)(((int64_t)a->n + P.S - 1) / P.S);
   P.slices = (a->hidden + 2047) / 2048;
-  const int64_t grid = (int64_t)P.tiles * P.slices + ((int64_t)a->vocab + EG_FILL_ROWS - 1) / EG_FILL_ROWS;
+  const int64_t row_bytes = (int64_t)a->hidden * elem_bytes(a->out_dtype);
+  P.fill_rows = row_bytes < EG_FILL ? (int)(EG_FILL / row_bytes) : 1;
+  const int64_t grid = (int64_t)P.tiles * P.slices + ((int64_t)a->vocab + P.fill_rows - 1) / P.fill_rows;
   if (grid > 0x7FFFFFFF || (a->hidden + 255) / 256 > 65535) return LPS_EINVAL;
   P.count = reinterpret_cast<int*>(ws + w.count);
   P.sid = reinterpret_cast<int*>(ws + w.sid);

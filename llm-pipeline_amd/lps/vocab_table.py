@@ -253,9 +253,9 @@ def embedding_grad(ids: torch.Tensor, grad: torch.Tensor, vocab: int, scale: flo
             raise ValueError("out requires a gradient; pass its .grad, or a detached tensor")
         res = out
     need = _lib.load().lps_embedding_grad_workspace_bytes(n, vocab, hidden)
-    ws = torch.empty((need,), dtype=torch.uint8, device=device)
+    ws = torch.empty((need,), dtype=torch.uint8, device=device) if need else None
     _call("lps_embedding_grad",
           _pack_grad(flat.data_ptr(), g.data_ptr(), res.data_ptr(), flat.element_size(), code, out_code, n, vocab, hidden,
                      g.stride(0) if n > 1 else hidden, res.stride(0) if vocab > 1 else hidden, scale,
-                     0 if out is None else 1, ws.data_ptr(), need), device)
+                     0 if out is None else 1, D.ptr(ws), need), device)
     return res

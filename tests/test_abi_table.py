@@ -63,9 +63,9 @@ def test_embedding_grad_argument_errors(lib, kw, code):  # noqa: F811
     from lps import _lib
     a = _lib.EmbeddingGradArgs()
     a.ids, a.grad, a.out, a.workspace = 0x1000, 0x2000, 0x3000, 0x4000
-    a.id_bytes, a.dtype, a.out_dtype, a.n, a.vocab, a.hidden = 8, 1, 0, 3, 10, 64
+    a.id_bytes, a.dtype, a.out_dtype, a.n, a.vocab, a.hidden = 8, 1, 0, 3000, 10, 64
     a.grad_stride = a.out_stride = 64
-    a.workspace_bytes = lib.lps_embedding_grad_workspace_bytes(3, 10, 64)
+    a.workspace_bytes = lib.lps_embedding_grad_workspace_bytes(3000, 10, 64)
     for k, v in kw.items():
         setattr(a, k, v)
     assert lib.lps_embedding_grad(ctypes.byref(a), None) == code
@@ -96,7 +96,9 @@ def test_lm_head_mx4_argument_errors(lib, kw, code):  # noqa: F811
 def test_workspace_bytes(lib):  # noqa: F811
     f = lib.lps_embedding_grad_workspace_bytes
     assert f(-1, 10, 10) == f(3, 0, 10) == f(3, 10, 0) == 0
-    assert 0 < f(0, 10, 10) <= f(100, 10, 10) <= f(100, 10, 1000) <= f(100000, 10, 1000)
+    assert f(0, 10, 10) == f(2048, 151936, 4096) == 0             # one launch, no workspace
+    assert 0 < f(2049, 10, 10) <= f(2049, 10, 1000) <= f(100000, 10, 1000)
+    assert f(5, 1 << 30, 8) > 0
 
 
 def test_cpu_tensors_are_refused():
