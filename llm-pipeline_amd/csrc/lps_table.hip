@@ -33,7 +33,10 @@ hipError_t launch_gather(GatherParams P, hipStream_t s) {
   // few rows: a long row over several workgroups
   const int chunks = (pieces + (1 << P.lg_tpr) - 1) >> P.lg_tpr;
   const unsigned y = wgs < 1024 ? (unsigned)(chunks < 65535 ? chunks : 65535) : 1u;
-  hipLaunchKernelGGL((gather_kernel<TDT, ODT>), dim3((unsigned)wgs, y), dim3(256), 0, s, P);
+  if (P.n * P.hidden * ElemBytes<ODT>::value > MX4_STREAM)
+    hipLaunchKernelGGL((gather_kernel<TDT, ODT, true>), dim3((unsigned)wgs, y), dim3(256), 0, s, P);
+  else
+    hipLaunchKernelGGL((gather_kernel<TDT, ODT, false>), dim3((unsigned)wgs, y), dim3(256), 0, s, P);
   return hipGetLastError();
 }
 template <int TDT>
@@ -43,6 +46,15 @@ hipError_t dispatch_gather(int out_dtype, const GatherParams& P, hipStream_t s) 
     case LPS_DTYPE_BF16: return launch_gather<TDT, LPS_DTYPE_BF16>(P, s);
     default: return launch_gather<TDT, LPS_DTYPE_F16>(P, s);
   }
+}
+
+template <int DT>
+hipError_t launch_quantize(Mx4Params P, hipStream_t s) {
+  P.lg_tpr = lg_threads_per_row(4 * P.blocks);
+  const dim3 grid((unsigned)(((int64_t)P.rows + (256 >> P.lg_tpr) - 1) >> (8 - P.lg_tpr)));
+  if ((int64_t)P.rows * P.blocks * 16 > MX4_STREAM) hipLaunchKernelGGL((mx4_quantize_kernel<DT, true>), grid, dim3(256), 0, s, P);
+  else hipLaunchKernelGGL((mx4_quantize_kernel<DT, false>), grid, dim3(256), 0, s, P);
+  return hipGetLastError();
 }
 
 int check_mx4(const lps_mx4_args* a) {
@@ -138,15 +150,11 @@ int lps_mx4_quantize(const lps_mx4_args* a, void* stream) {
   P.codes_stride = a->rows > 1 ? a->codes_stride : 0;
   P.scales_stride = a->rows > 1 ? a->scales_stride : 0;
   P.words = aligned_to(a->scales, 4) && P.scales_stride % 4 == 0;
-  P.lg_tpr = lg_threads_per_row(4 * P.blocks);
-  const dim3 grid((unsigned)(((int64_t)a->rows + (256 >> P.lg_tpr) - 1) >> (8 - P.lg_tpr)));
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  switch (a->dtype) {
-    case LPS_DTYPE_F32: hipLaunchKernelGGL((mx4_quantize_kernel<LPS_DTYPE_F32>), grid, dim3(256), 0, s, P); break;
-    case LPS_DTYPE_BF16: hipLaunchKernelGGL((mx4_quantize_kernel<LPS_DTYPE_BF16>), grid, dim3(256), 0, s, P); break;
-    default: hipLaunchKernelGGL((mx4_quantize_kernel<LPS_DTYPE_F16>), grid, dim3(256), 0, s, P); break;
-  }
-  return hipGetLastError() == hipSuccess ? LPS_OK : LPS_ELAUNCH;
+  const hipError_t e = a->dtype == LPS_DTYPE_F32 ? launch_quantize<LPS_DTYPE_F32>(P, s)
+                       : a->dtype == LPS_DTYPE_BF16 ? launch_quantize<LPS_DTYPE_BF16>(P, s)
+                                                    : launch_quantize<LPS_DTYPE_F16>(P, s);
+  return e == hipSuccess ? LPS_OK : LPS_ELAUNCH;
 }
 
 int lps_mx4_dequantize(const lps_mx4_args* a, void* stream) {

@@ -93,8 +93,13 @@ def _same_device(a: torch.Tensor, b: torch.Tensor, what: str) -> None:
 
 
 def _call(name: str, args: bytes, device: torch.device) -> None:
-    with D.guard(device):
-        rc = getattr(_lib.load(), name)(args, D.stream_of(device))
+    """The entry point on the device's current stream; raises for its return code."""
+    fn = getattr(_lib.load(), name)
+    if torch._C._cuda_getDevice() == device.index:
+        rc = fn(args, torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with D.guard(device):
+            rc = fn(args, D.stream_of(device))
     if rc:
         _lib.check(rc, name)
 
