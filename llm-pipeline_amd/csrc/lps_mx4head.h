@@ -15,6 +15,15 @@
 // scale a lane.  bf16 holds every value of w.  fp16 holds those of scales 2^-23 ..
 // 2^13; a stage in which a wave meets another scale takes x apart into two bf16
 // (11 bits as 8 and 3) and runs the bf16 instruction twice, which is exact too.
+//
+// What bounds it: up to ~32 rows w's pass over HBM (1 row of 4096 -> 151936: 58 us, 5.7
+// TB/s; a read reaches 7.0), from ~128 rows of 16 bits the matrix cores (2048 rows 2.15
+// ms, 1.19 PFLOP/s; the library's bf16 product takes 2.10) and from ~256 of 4 bits they
+// and the writing of the logits (2048 rows 764 us, 3.3 PFLOP/s).  Between them (64 rows
+// of 16 bits 101 us) stages of x and w wait for each other's latency: two workgroups of
+// 72 KB LDS on a CU are worth more than a deeper ring in one (64 x 128 tiles with 5
+// stages of w ahead 120 us; 64 x 256 tiles 111), and so are x held in registers with w
+// streamed past it (155) and a stage read whole into registers, a stage ahead (101).
 #pragma once
 
 #include <type_traits>
@@ -295,10 +304,6 @@ __global__ __launch_bounds__(T::NTK, T::WPE) void mx4head_kernel(Mx4HeadParams Q
   auto mrow = [&](int r) { return m0 + r < P.M ? r : P.M - 1 - m0; };
   auto nrow = [&](int r) { return n0 + r < P.V ? r : P.V - 1 - n0; };
 
-  // (128 accumulators, two sets of fragments and the loads' offsets do not fit a
-  // wave's 256 registers: there a step reads its own fragments, the other wave of
-  // the SIMD fills the gap, and offsets are computed when they are needed)
-  constexpr bool AHEAD = !(T::XS && MT * CT >= 8 && T::WPE > 1);
   // offsets of this lane's chunk of the k-th row that its wave loads: rows k R + rl, R
   // a multiple of 8 (so that the place in the row is the same), clamped to the last
   const int rl = loads_x ? lw % T::XI * T::XRI + l / T::XC : lw * T::WRI + l / T::WC;
@@ -308,8 +313,9 @@ __global__ __launch_bounds__(T::NTK, T::WPE) void mx4head_kernel(Mx4HeadParams Q
   const uint32_t roff = (uint32_t)rl * rstep;
   const uint32_t coff = (uint32_t)(loads_x ? (l % T::XC) ^ T::xperm(rl) : (l % T::WC) ^ T::wperm(rl)) * 16u;
   constexpr int LPM = T::XPW > T::WPW ? T::XPW : T::WPW;
-  uint32_t offs[AHEAD ? LPM : 1];
-  if constexpr (AHEAD) {
+  constexpr bool KEEP = !(T::XS && MT * CT >= 8);   // (beside 128 accumulators computed when they are needed)
+  uint32_t offs[KEEP ? LPM : 1];
+  if constexpr (KEEP) {
 #pragma unroll
     for (int k = 0; k < LPM; k++) {
       const uint32_t o = roff + (uint32_t)k * rnext;
@@ -317,7 +323,7 @@ __global__ __launch_bounds__(T::NTK, T::WPE) void mx4head_kernel(Mx4HeadParams Q
     }
   }
   auto off = [&](int k) {
-    if constexpr (AHEAD) return offs[k];
+    if constexpr (KEEP) return offs[k];
     uint32_t o = roff;
     LPS_KEEP_VGPR(o);
     o += (uint32_t)k * rnext;
@@ -358,21 +364,17 @@ __global__ __launch_bounds__(T::NTK, T::WPE) void mx4head_kernel(Mx4HeadParams Q
 
   typename MfmaOps<ADT>::acc acc[MT][CT] = {};
   const M4Lane<T> L(wv, l);
-  // Fragments are (AHEAD) read one step ahead of their matrix instructions and, of a
-  // 16-bit x, the codes converted one ahead, in the shadow of the matrix cores;
-  // the last step of a stage waits for the next one and reads its first.
   constexpr int STEPS = T::XS ? JS : 4 * JS;       // matrix steps of a wave in an x stage (64 or 16 values)
-  constexpr int WDS = XNB / 4;               // words of scales of an x stage
+  constexpr int WDS = T::XS ? 1 : XNB / 4;         // words of scales that are held
   u32x4 fx[2][MT], cw[2][CT], fw[2][CT];
-  uint32_t sw[WDS][CT], sx[WDS][MT];
+  uint32_t sw[WDS][CT], sx[MT];
   // pair jj of a wave is pair jj KW + kg of the stage: word and (after the shift)
   // byte of its scales
   auto word = [](int jj) { return KW == 2 ? jj : jj >> 1; };
   auto odd = [](int jj) { return KW == 2 ? 0 : jj & 1; };
   const int shift = 8 * L.half + (KW == 2 ? 16 * L.kg : 0);
   uint32_t far_any = 0;                            // fp16: whether this lane met a scale that it does not hold
-  auto read_word = [&](const char* scales, int w0, int d, int to) {
-    d += w0 >> 2;
+  auto read_word = [&](const char* scales, int d, int to) {
 #pragma unroll
     for (int i = 0; i < CT; i++) {
       const uint32_t w = L.wscales(scales, i, d);
@@ -381,15 +383,13 @@ __global__ __launch_bounds__(T::NTK, T::WPE) void mx4head_kernel(Mx4HeadParams Q
     }
     if constexpr (T::XS) {
 #pragma unroll
-      for (int i = 0; i < MT; i++) sx[to][i] = L.xscales(scales, i, d) >> shift;
+      for (int i = 0; i < MT; i++) sx[i] = L.xscales(scales, i, d) >> shift;
     }
   };
   auto read_scales = [&](const char* scales, int w0) {
     far_any = 0;
-    if constexpr (AHEAD) {
 #pragma unroll
-      for (int d = 0; d < WDS; d++) read_word(scales, w0, d, d);
-    }
+    for (int d = 0; d < WDS; d++) read_word(scales, (w0 >> 2) + d, d);
   };
   // (b: the buffer of registers)
   auto read_x = [&](const char* xs, int k, int b) {   // for matrix step k
@@ -414,110 +414,113 @@ __global__ __launch_bounds__(T::NTK, T::WPE) void mx4head_kernel(Mx4HeadParams Q
   if (ns > 0) {
     if (loads_x) {
       for (int i = 0; i < T::NSX && i < its; i++) issue_x(i, i);
-      m4_wait_left<T::XPW, T::NSX - 1>(its - 1);
     } else {
       issue_scales(0);
       for (int s = 0; s < T::NSW && s < ns; s++) issue_w(s, s);
-      m4_wait_left<T::WPW, T::NSW - 1>(ns - 1);
     }
-    m4_barrier();
-    read_scales(scales_of(0), 0);
-    if constexpr (AHEAD) {
+    int xb = 0, wb = 0;                            // the places of x stage i and of its w stage
+    // until x stage i (and the w stage that it begins, and its scales, asked for before
+    // it) has landed, with up to MORE stages after it in flight, for every wave
+    auto wait_stage = [&](int i, auto more_c) {
+      constexpr int MORE = decltype(more_c)::value;
+      if (loads_x) m4_wait_left<T::XPW, T::NSX - MORE>(its - 1 - i);
+      else if (i % T::ITS == 0) m4_wait_left<T::WPW, T::NSW - MORE>(ns - 1 - i / T::ITS);
+      m4_barrier();
+    };
+    // every wave is done with x stage i: the next ones into its places
+    auto refill = [&](int i, int xplace, int wplace) {
+      if (loads_x) {
+        if (i + T::NSX < its) issue_x(i + T::NSX, xplace);
+      } else if ((i + 1) % T::ITS == 0) {
+        const int s = i / T::ITS;
+        if (s % M4_PER == 0 && s + M4_PER < ns) issue_scales(s / M4_PER + 1);
+        if (s + T::NSW < ns) issue_w(s + T::NSW, wplace);
+      }
+    };
+    constexpr std::integral_constant<int, 1> first{};   // (the ring is full)
+    constexpr std::integral_constant<int, 2> later{};   // (but for the stage that has just been read)
+    if constexpr (T::XS) {
+      // A step reads its own fragments; the compiler moves the next ones' reads up among
+      // its matrix instructions as registers allow.
+      for (int i = 0; i < its; i++) {
+        if (i == 0) wait_stage(0, first);
+        else wait_stage(i, later);
+        if (i > 0) refill(i - 1, xb == 0 ? T::NSX - 1 : xb - 1, wb == 0 ? T::NSW - 1 : wb - 1);
+        const char* const xs = xslot(xb);
+        const char* const ws = wslot(wb);
+        static_assert(!T::XS || T::ITS == 1, "4-bit x: a w stage to an x stage");
+#pragma unroll
+        for (int k = 0; k < STEPS; k++) {
+          read_w(ws, 0, k, 0);
+          read_x(xs, k, 0);
+          if (!odd(k)) read_word(scales_of(i), word(k), 0);
+#pragma unroll
+          for (int a = 0; a < MT; a++)
+#pragma unroll
+            for (int b = 0; b < CT; b++) acc[a][b] = m4_mma4(fx[0][a], cw[0][b], acc[a][b], sx[a], sw[0][b], odd(k));
+        }
+        xb = xb + 1 == T::NSX ? 0 : xb + 1;
+        wb = wb + 1 == T::NSW ? 0 : wb + 1;
+      }
+    } else {
+      // Fragments are read one step ahead of their matrix instructions and the codes
+      // converted one ahead, in the shadow of the matrix cores; the last step of a stage
+      // waits for the next one and reads its first.  (With all of a stage read at once, a
+      // stage ahead: 8 rows 74 us for 59, 64 rows 101 for 101.)
+      wait_stage(0, first);
+      read_scales(scales_of(0), 0);
       read_w(wslot(0), 0, 0, 0);
       read_x(xslot(0), 0, 0);
       convert(0, 0, 0);
-    }
-    int xb = 0, wb = 0;
-    // every wave holds its last fragments of stage i, stage i + 1 has landed (and its
-    // scales, asked for before it)
-    auto next_stage = [&](int i, int s, bool next_w) {
-      if (loads_x) m4_wait_left<T::XPW, T::NSX - 2>(its - 2 - i);
-      else if (next_w) m4_wait_left<T::WPW, T::NSW - 2>(ns - 2 - s);
-      m4_barrier();
-      if (loads_x) {
-        if (i + T::NSX < its) issue_x(i + T::NSX, xb);
-      } else if (next_w) {
-        if (s % M4_PER == 0 && s + M4_PER < ns) issue_scales(s / M4_PER + 1);
-        if (s + T::NSW < ns) issue_w(s + T::NSW, wb);
-      }
-      read_scales(scales_of((i + 1) / T::ITS), (i + 1) % T::ITS * XNB);
-    };
-    // (an odd number of pairs a stage: the buffers of registers swap from stage to stage)
-    auto stage = [&](int i, auto par_c) {
-      constexpr int PAR = decltype(par_c)::value;  // the buffer of the stage's first codes (4 bits: and fragments)
-      const int w0 = (i % T::ITS) * XNB, s = i / T::ITS;
-      const char* const xs = xslot(xb);
-      const char* const ws = wslot(wb);
-      const bool far = XDT == LPS_DTYPE_F16 && wballot(far_any != 0) != 0;   // (uniform over the wave)
-      if (XDT == LPS_DTYPE_F16 && far) m4_plain_stage<XDT, T, true>(xs, ws, w0, scales_of(s), L, acc, XNB / 2);
-      const int nxb = xb + 1 == T::NSX ? 0 : xb + 1;
-      const bool next_w = (i + 1) % T::ITS == 0;
-      const int nwb = !next_w ? wb : wb + 1 == T::NSW ? 0 : wb + 1;
+      // (an odd number of pairs a stage: the buffers of codes swap from stage to stage)
+      auto stage = [&](int i, auto par_c) {
+        constexpr int PAR = decltype(par_c)::value;  // the buffer of the stage's first codes
+        const int w0 = (i % T::ITS) * XNB, s = i / T::ITS;
+        const char* const xs = xslot(xb);
+        const char* const ws = wslot(wb);
+        const bool far = XDT == LPS_DTYPE_F16 && wballot(far_any != 0) != 0;   // (uniform over the wave)
+        if constexpr (XDT == LPS_DTYPE_F16)
+          if (far) m4_plain_stage<XDT, T, true>(xs, ws, w0, scales_of(s), L, acc, XNB / 2);
+        const int nxb = xb + 1 == T::NSX ? 0 : xb + 1;
+        const int nwb = (i + 1) % T::ITS != 0 ? wb : wb + 1 == T::NSW ? 0 : wb + 1;
 #pragma unroll
-      for (int k = 0; k < STEPS; k++) {
-        const int jj = T::XS ? k : k >> 2;
-        const int fb = T::XS ? (k + PAR) & 1 : k & 1, fn = fb ^ 1;             // fragments of this step, the next one's
-        const int cb = (jj + PAR) & 1, cn = cb ^ 1;                            // codes of this pair, the next one's
-        if constexpr (!AHEAD) {
-          read_w(ws, w0, k, 0);
-          read_x(xs, k, 0);
-          if (!odd(jj)) read_word(scales_of(s), w0, word(jj), 0);
-#pragma unroll
-          for (int a = 0; a < MT; a++)
-#pragma unroll
-            for (int b = 0; b < CT; b++)
-              acc[a][b] = m4_mma4(fx[0][a], cw[0][b], acc[a][b], sx[0][a], sw[0][b], odd(jj));
-          if (k + 1 == STEPS && i + 1 < its) next_stage(i, s, next_w);
-        } else if (k + 1 < STEPS) {
-          if (XDT == LPS_DTYPE_F16 && far) continue;
-          if constexpr (T::XS) read_w(ws, w0, k + 1, cn);
-          else if ((k & 3) == 1 && jj + 1 < JS) read_w(ws, w0, jj + 1, cn);
-          read_x(xs, k + 1, fn);
-          __builtin_amdgcn_sched_barrier(0);   // (the compiler would move the reads down to their use)
-#pragma unroll
-          for (int a = 0; a < MT; a++)
-#pragma unroll
-            for (int b = 0; b < CT; b++) {
-              if constexpr (T::XS) acc[a][b] = m4_mma4(fx[fb][a], cw[cb][b], acc[a][b], sx[word(jj)][a], sw[word(jj)][b], odd(jj));
-              else acc[a][b] = MfmaOps<ADT>::mma(fx[fb][a], fw[fb][b], acc[a][b]);
-            }
-          convert(k + 1, ((k + 1) >> 2) == jj ? cb : cn, fn);
-          __builtin_amdgcn_sched_barrier(0);
-        } else {
-          uint32_t ow[CT], ox[MT];             // (this step's scales)
-          if constexpr (T::XS) {
-#pragma unroll
-            for (int b = 0; b < CT; b++) ow[b] = sw[word(jj)][b];
-#pragma unroll
-            for (int a = 0; a < MT; a++) ox[a] = sx[word(jj)][a];
-          }
-          if (i + 1 < its) {
-            next_stage(i, s, next_w);
+        for (int k = 0; k < STEPS; k++) {
+          const int jj = k >> 2;
+          const int fb = k & 1, fn = fb ^ 1;         // fragments of this step, the next one's
+          const int cb = (jj + PAR) & 1, cn = cb ^ 1;   // codes of this pair, the next one's
+          if (k + 1 < STEPS) {
+            if (far) continue;
+            if ((k & 3) == 1 && jj + 1 < JS) read_w(ws, w0, jj + 1, cn);
+            read_x(xs, k + 1, fn);
+          } else if (i + 1 < its) {
+            // (every wave holds its last fragments of the stage)
+            wait_stage(i + 1, later);
+            refill(i, xb, wb);
+            read_scales(scales_of((i + 1) / T::ITS), (i + 1) % T::ITS * XNB);
             read_w(wslot(nwb), ((i + 1) % T::ITS) * XNB, 0, cn);
             read_x(xslot(nxb), 0, fn);
-            __builtin_amdgcn_sched_barrier(0);
           }
-          if (!(XDT == LPS_DTYPE_F16 && far)) {
+          __builtin_amdgcn_sched_barrier(0);   // (the compiler would move the reads down to their use)
+          if (!far) {
 #pragma unroll
             for (int a = 0; a < MT; a++)
 #pragma unroll
-              for (int b = 0; b < CT; b++) {
-                if constexpr (T::XS) acc[a][b] = m4_mma4(fx[fb][a], cw[cb][b], acc[a][b], ox[a], ow[b], odd(jj));
-                else acc[a][b] = MfmaOps<ADT>::mma(fx[fb][a], fw[fb][b], acc[a][b]);
-              }
+              for (int b = 0; b < CT; b++) acc[a][b] = MfmaOps<ADT>::mma(fx[fb][a], fw[fb][b], acc[a][b]);
           }
-          if (i + 1 < its) convert(0, cn, fn);
+          if (k + 1 < STEPS) convert(k + 1, ((k + 1) >> 2) == jj ? cb : cn, fn);
+          else if (i + 1 < its) convert(0, cn, fn);
+          __builtin_amdgcn_sched_barrier(0);
         }
-      }
-      xb = nxb;
-      wb = nwb;
-    };
-    if constexpr (JS % 2 == 0 || !AHEAD) {
-      for (int i = 0; i < its; i++) stage(i, std::integral_constant<int, 0>{});
-    } else {
-      for (int i = 0; i < its; i += 2) {
-        stage(i, std::integral_constant<int, 0>{});
-        if (i + 1 < its) stage(i + 1, std::integral_constant<int, 1>{});
+        xb = nxb;
+        wb = nwb;
+      };
+      if constexpr (JS % 2 == 0) {
+        for (int i = 0; i < its; i++) stage(i, std::integral_constant<int, 0>{});
+      } else {
+        for (int i = 0; i < its; i += 2) {
+          stage(i, std::integral_constant<int, 0>{});
+          if (i + 1 < its) stage(i + 1, std::integral_constant<int, 1>{});
+        }
       }
     }
     m4_barrier();

@@ -24,10 +24,10 @@ hipError_t launch_mx4head(Mx4HeadParams Q, hipStream_t s) {
 // 46; 256 of 8192 25, 26, 48; 512 of 8192 47, 40, 60; 1024 of 8192 94, 78, 62; 128 of
 // 32000 45, 41, 50; 256 of 32000 85, 76, 58; 64 of 151936 -, 95, 160.  x in 4 bits:
 // 256 rows of V 8192 -, 13, 18, 35; 512 of 8192 -, 24, 21, 38; 1024 of 8192 -, 42, 29,
-// 40; 512 of 32000 -, 80, 49, 44; 512 of 151936 -, -, 258, 267; 2048 -, -, 956, 853.
+// 40; 512 of 32000 -, 80, 47, 41; 512 of 151936 -, -, 251, 204; 2048 -, -, 964, 764.
 struct M4Shape { int bm, bn, per_cu, rows; };
 constexpr M4Shape M4_SHAPES16[] = {{32, 128, 2, 32}, {64, 128, 2, 64}, {128, 256, 1, 0}};
-constexpr M4Shape M4_SHAPES4[] = {{32, 128, 1, 32}, {64, 128, 1, 64}, {128, 128, 2, 256}, {256, 256, 1, 0}};
+constexpr M4Shape M4_SHAPES4[] = {{32, 128, 1, 32}, {64, 128, 1, 64}, {128, 128, 2, 128}, {256, 256, 1, 0}};
 template <int N>
 int mx4head_shape(const M4Shape (&shapes)[N], int M, int V, int cus) {
   for (int i = 0; i < N; i++) {
@@ -44,7 +44,7 @@ hipError_t launch_mx4head_rows(const Mx4HeadParams& Q, hipStream_t s) {
     switch (mx4head_shape(M4_SHAPES4, M, V, cus)) {
       case 0: return launch_mx4head<XDT, ODT, M4Tile<32, 128, 1, 4, 2, 8, 2, 2, 4, 2, 16>, true>(Q, s);
       case 1: return launch_mx4head<XDT, ODT, M4Tile<64, 128, 2, 2, 2, 8, 2, 2, 4, 2, 16>, true>(Q, s);
-      case 2: return launch_mx4head<XDT, ODT, M4Tile<128, 128, 2, 2, 1, 8, 2, 2, 2, 1, 16>, false>(Q, s);
+      case 2: return launch_mx4head<XDT, ODT, M4Tile<128, 128, 2, 4, 1, 8, 2, 2, 4, 4, 16>, false>(Q, s);
       default: return launch_mx4head<XDT, ODT, M4Tile<256, 256, 2, 4, 1, 8, 2, 2, 4, 2, 16>, false>(Q, s);
     }
   } else {
