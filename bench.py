@@ -633,6 +633,72 @@ def lm_head_bench(args):
     }), flush=True)
 
 
+def vocab_table_bench(args):
+    """A decode step through the vocabulary table alone (the model's layers
+    between its two ends left out): the sampled tokens' rows (``embedding``), their
+    products with every row (``lm_head``), the next tokens (``sample_rows``), 64
+    requests, V = 151936, H = 4096, with the table in 4 bits and in bf16; and a
+    training step's share of it: 8192 tokens' gradients added to 32-bit sums
+    (``embedding_grad``), the table stepped and quantised again."""
+    import torch
+    from lps import SamplingParams, embedding, embedding_grad, lm_head, mx4_quantize, sample_rows
+
+    dev = torch.device("cuda:0")
+    torch.cuda.set_device(dev)
+    g = torch.Generator(device=dev).manual_seed(0)
+    B, V, H, N = 64, 151936, 4096, 8192
+    w = torch.randn((V, H), generator=g, device=dev, dtype=torch.bfloat16).mul_(0.02)
+    w4 = mx4_quantize(w)
+    params = SamplingParams.build(B, dev, temperature=0.8, top_k=50, top_p=0.95)
+    steps = max(20, min(args.steps, 500))
+    us = torch.rand((steps, B), generator=g, device=dev)
+
+    def decode(table):
+        ids = torch.randint(0, V, (B,), generator=g, device=dev)
+        for s in range(steps):
+            logits = lm_head(embedding(ids, table, scale=H ** 0.5, out_dtype=torch.bfloat16), table)
+            ids = sample_rows(logits, params, us[s]).tokens
+        return ids
+
+    def timed(fn, n):
+        fn()
+        torch.cuda.synchronize()
+        e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        e0.record()
+        fn()
+        e1.record()
+        torch.cuda.synchronize()
+        return e0.elapsed_time(e1) / n
+
+    t4, t16 = timed(lambda: decode(w4), steps), timed(lambda: decode(w), steps)
+    tokens = torch.randint(0, V, (N,), generator=g, device=dev)
+    grad = torch.randn((N, H), generator=g, device=dev, dtype=torch.bfloat16)
+    sums = torch.zeros((V, H), device=dev)
+
+    def train():
+        embedding_grad(tokens, grad, V, scale=H ** 0.5, out=sums)
+        w.add_(sums, alpha=-1e-4)
+        sums.zero_()
+        return mx4_quantize(w)
+
+    t_train = timed(train, 1)
+    row4 = H // 32 * 17
+    abytes = V * row4 + B * (row4 + 2 * H) + 2 * B * V * 2      # the table, the rows looked up, the logits out and in
+    gbs = abytes / (t4 / 1e3) / 1e9
+    print(json.dumps({
+        "metric": "Decode step through a 4-bit vocabulary table (lookup, LM head, sampling), rows/s at B=64, V=151936, H=4096",
+        "value": round(B / t4 * 1e3, 1), "unit": "rows/s", "n_gpus": 1, "steps": steps, "warmup": steps,
+        "ms_per_step": round(t4, 5), "higher_is_better": True, "scaling": "weak", "vs_baseline": None,
+        "dtype": "4-bit weight, bf16 states, f32 accumulate", "data": "synthetic",
+        "bf16_table_ms": round(t16, 5), "table_step_ms": round(t_train, 5),
+        "config": {"workload": "64 requests, top_k 50, top_p 0.95, T 0.8; table_step: 8192 tokens' gradients into "
+                               "32-bit sums, the table stepped, quantised to 4 bits",
+                   "algorithmic_bytes_per_step": abytes},
+        "roofline": {"bound": "hbm", "achieved": round(gbs, 1), "peak": PEAK_HBM_GBS, "unit": "GB/s",
+                     "frac": round(gbs / PEAK_HBM_GBS, 4)},
+    }), flush=True)
+
+
 def spec_bench(args):
     """c4: speculative-decoding verification (``lps_spec_verify``, the drop-in
     for ``speculative.py:119-174``): 32 requests, k = 4, target logits
@@ -753,7 +819,12 @@ def main():
                     help="time the batched speculative-decoding driver (zero-cost synthetic forwards)")
     ap.add_argument("--lm-head", action="store_true",
                     help="time the LM-head projection with the softmax statistics epilogue")
+    ap.add_argument("--vocab-table", action="store_true",
+                    help="time a decode step through a 4-bit vocabulary table (lookup, LM head, sampling)")
     args = ap.parse_args()
+    if args.vocab_table:
+        vocab_table_bench(args)
+        return
     if args.lm_head:
         lm_head_bench(args)
         return

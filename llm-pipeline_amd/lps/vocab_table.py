@@ -1,12 +1,12 @@
 """The vocabulary table's operators on the GPU.
 
 A decode loop uses one table ``[V, H]`` at both of its ends: the sampled
-token's row goes in (the reference's ``nn.Embedding``,
-``models/qwen3/custom_builder.py``) and the hidden state's products with every
-row come out (``lm_head``, the same file ``:415``).  ``embedding`` looks rows
-up, ``embedding_grad`` is its gradient, and ``mx4_quantize`` gives the table's
-form in microscaled 4-bit floats (17/64 of its bf16 bytes), which
-``embedding`` and ``lm_head`` take in the table's place."""
+token's row goes in, and the hidden state's products with every row come out
+(the reference's ``lm_head``, ``models/qwen3/custom_builder.py:415``).
+``embedding`` looks rows up, ``embedding_grad`` is its gradient, and
+``mx4_quantize`` gives the table's form in microscaled 4-bit floats (17/64 of
+its bf16 bytes), which ``embedding`` and ``lm_head`` take in the table's
+place."""
 
 from __future__ import annotations
 
