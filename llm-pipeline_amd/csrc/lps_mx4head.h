@@ -81,14 +81,15 @@ struct M4Tile {
   static constexpr int ITS = M4_NB / XNB;                       // x stages to one of w
   static constexpr int JS = XNB / 2 / KW;                       // pairs of blocks of a wave per x stage
   static_assert(XNB == 4 || XNB == 8, "x stages");
-  static_assert(NXW * XRI % 8 == 0 || XPW == 1, "the rows of a lane's loads share their permutation");
   static_assert((XI % NXW == 0 || NXW % XI == 0) && WI % NWW == 0 && NXW < NWK, "whole load instructions per wave");
   static_assert(SROWS % 32 == 0 && XR % 8 == 0 && BM % XR == 0, "whole loads of scales");
   static_assert(BM % (32 * WM) == 0 && BN % (32 * WN) == 0 && BN % LMH_BN == 0 && JS >= 1, "tile shape");
   static_assert(M4_PER >= NSW - 1, "scales are asked for before the stage that needs them");
   static_assert((NSW - 1) * WPW + SROWS / 8 / NWW + 1 < 64 && (NSX - 1) * XPW < 64, "the load counter holds 63");
-  __device__ __forceinline__ static int xperm(int row) { return XC >= 8 ? (row & 7) : ((row >> 1) & 3); }
-  __device__ __forceinline__ static int wperm(int row) { return row & 7; }
+  // (the 64 banks hold 16 chunks: those that 16 neighbouring rows read at once lie in
+  // places of their own; of 128-byte rows two share the banks)
+  __device__ __forceinline__ static int xperm(int row) { return XC >= 16 ? (row & 15) : ((row >> 1) & 7); }
+  __device__ __forceinline__ static int wperm(int row) { return (row >> 1) & 7; }
 };
 // The waves that write a tile out, as lmh_epilogue sees them.
 template <typename T>
@@ -210,7 +211,7 @@ struct M4Lane {
     kg = wv / T::EW;
     xr = (e / T::WN) * (T::MT * 32) + (l & 31);
     wr = (e % T::WN) * T::WTN + (l & 31);
-    px = T::xperm(xr % T::XR);      // (rows 32 apart share their permutation)
+    px = T::xperm(xr % T::XR);      // (rows 32 apart share it)
     pw = T::wperm(wr);
   }
   __device__ __forceinline__ u32x4 x(const char* xs, int i, int c) const {
@@ -304,30 +305,30 @@ __global__ __launch_bounds__(T::NTK, T::WPE) void mx4head_kernel(Mx4HeadParams Q
   auto mrow = [&](int r) { return m0 + r < P.M ? r : P.M - 1 - m0; };
   auto nrow = [&](int r) { return n0 + r < P.V ? r : P.V - 1 - n0; };
 
-  // offsets of this lane's chunk of the k-th row that its wave loads: rows k R + rl, R
-  // a multiple of 8 (so that the place in the row is the same), clamped to the last
+  // offsets of this lane's chunk of the k-th row that its wave loads, rl + k R, clamped
+  // to the last row
+  constexpr int RX = T::NXW * T::XRI, RW = T::NWW * T::WRI, LPM = T::XPW > T::WPW ? T::XPW : T::WPW;
+  constexpr bool KEEP = !(T::XS && MT * CT >= 8);   // (beside 128 accumulators computed when they are needed)
+  static_assert(KEEP || (RX % 16 == 0 && RW % 16 == 0), "there the rows share their chunk's place");
   const int rl = loads_x ? lw % T::XI * T::XRI + l / T::XC : lw * T::WRI + l / T::WC;
   const uint32_t rstep = loads_x ? (uint32_t)xstep : (uint32_t)P.w_stride;
-  const uint32_t rnext = rstep * (uint32_t)(loads_x ? T::NXW * T::XRI : T::NWW * T::WRI);
   const uint32_t rlast = (uint32_t)(loads_x ? mrow(T::XR - 1) : nrow(T::BN - 1)) * rstep;
   const uint32_t roff = (uint32_t)rl * rstep;
-  const uint32_t coff = (uint32_t)(loads_x ? (l % T::XC) ^ T::xperm(rl) : (l % T::WC) ^ T::wperm(rl)) * 16u;
-  constexpr int LPM = T::XPW > T::WPW ? T::XPW : T::WPW;
-  constexpr bool KEEP = !(T::XS && MT * CT >= 8);   // (beside 128 accumulators computed when they are needed)
+  auto chunk = [&](int row) { return (uint32_t)(loads_x ? (l % T::XC) ^ T::xperm(row) : (l % T::WC) ^ T::wperm(row)) * 16u; };
+  auto compute = [&](int k) {
+    uint32_t o = roff;
+    if constexpr (!KEEP) LPS_KEEP_VGPR(o);
+    o += (uint32_t)k * rstep * (uint32_t)(loads_x ? RX : RW);
+    return (o < rlast ? o : rlast) + chunk(KEEP ? rl + k * (loads_x ? RX : RW) : rl);
+  };
   uint32_t offs[KEEP ? LPM : 1];
   if constexpr (KEEP) {
 #pragma unroll
-    for (int k = 0; k < LPM; k++) {
-      const uint32_t o = roff + (uint32_t)k * rnext;
-      offs[k] = (o < rlast ? o : rlast) + coff;
-    }
+    for (int k = 0; k < LPM; k++) offs[k] = compute(k);
   }
   auto off = [&](int k) {
     if constexpr (KEEP) return offs[k];
-    uint32_t o = roff;
-    LPS_KEEP_VGPR(o);
-    o += (uint32_t)k * rnext;
-    return (o < rlast ? o : rlast) + coff;
+    else return compute(k);
   };
   const auto lds0 = m4_lds(lds);
   auto issue_x = [&](int i, int slot) {
