@@ -392,7 +392,7 @@ int lps_mx4_dequantize(const lps_mx4_args* args, void* stream);
  * x in bf16, fp16 or 4 bits.  Any hidden; the codes of w past a row's end count
  * as zeros, those of a 4-bit x must be (lps_mx4_quantize leaves them so).
  * Rows of x and w begin on 16-byte lines, rows of scales on 4-byte lines;
- * strides are at most 8 MiB. */
+ * strides are at most 8 MiB, vocab 2^21, hidden 2^24. */
 typedef struct lps_lm_head_mx4_args {
   const void* x;                  /* [rows, hidden] in dtype; 4-bit codes */
   const void* x_scales;           /* 4-bit x: uint8 [rows, ceil(hidden / 32)] */
@@ -440,7 +440,8 @@ int lps_embedding(const lps_embedding_args* args, void* stream);
  *   out[v] = scale * sum of grad[i] over the i with ids[i] = v
  * (ids outside [0, vocab) add nothing), on top of out[v] with accumulate (rows
  * without an id are then not touched).  Summed in fp32, rounded once, in an
- * order that depends on ids and sizes alone: equal calls give equal bits.
+ * order that depends on ids and sizes alone: equal calls give equal bits.  At most
+ * 2^30 positions.
  * workspace: lps_embedding_grad_workspace_bytes(n, vocab, hidden) bytes (0 for few
  * positions), 16-byte aligned, of any content; calls that overlap in time must not
  * share it. */

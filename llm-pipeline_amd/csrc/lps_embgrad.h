@@ -27,7 +27,7 @@ constexpr int EG_NT = 1024;         // threads of the sort
 constexpr int EG_NW = EG_NT / 64;
 constexpr int EG_OWN = 1024;        // ids a workgroup of the sort can own
 constexpr int EG_LIST = 4096;       // positions it keeps in LDS
-constexpr int EG_SMAX = 256;        // positions of a tile, at most
+constexpr int EG_SMAX = 1024;       // positions of a tile, at most
 constexpr int EG_FILL = 8192;       // bytes of rows that a zeroing workgroup looks at, or one row
 constexpr int EG_JOIN = 8;          // tiles a joining workgroup looks at
 constexpr int EG_SMALL = 2048;      // positions of the one-launch form

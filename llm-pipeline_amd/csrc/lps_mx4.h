@@ -21,6 +21,7 @@
 namespace lps {
 
 constexpr int MX4_BLOCK = 32;
+constexpr int MX4_MAX_HIDDEN = 1 << 24;   // of every operator on rows: offsets within one stay in 32 bits
 constexpr int64_t MX4_STREAM = 32 << 20;   // bytes: the card's L2s
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));

@@ -9,6 +9,9 @@ using namespace lps;
 
 namespace {
 
+// (131070 row tiles of 32 times 16383 column tiles of 128 are fewer than 2^31)
+constexpr int kMaxHeadVocab = 1 << 21;
+
 template <int XDT, int ODT, typename T, bool NTL>
 hipError_t launch_mx4head(Mx4HeadParams Q, hipStream_t s) {
   Q.h.mtiles = (Q.h.M + T::BM - 1) / T::BM;
@@ -81,7 +84,9 @@ extern "C" int lps_lm_head_mx4(const lps_lm_head_mx4_args* a, void* stream) {
   const bool x4 = a->dtype == LPS_DTYPE_MX4;
   if (!x4 && a->dtype != LPS_DTYPE_BF16 && a->dtype != LPS_DTYPE_F16) return LPS_EUNSUPPORTED_DTYPE;
   if (!dtype_ok(a->out_dtype)) return LPS_EUNSUPPORTED_DTYPE;
-  if (a->rows < 0 || a->vocab < 1 || a->hidden < 1 || a->rows > LMH_MAX_ROWS) return LPS_EINVAL;
+  if (a->rows < 0 || a->vocab < 1 || a->hidden < 1 || a->rows > LMH_MAX_ROWS || a->vocab > kMaxHeadVocab ||
+      a->hidden > MX4_MAX_HIDDEN)
+    return LPS_EINVAL;
   if (a->rows == 0) return LPS_OK;
   if (!a->x || !a->w || !a->w_scales || !a->out || (x4 && !a->x_scales)) return LPS_EINVAL;
   const int64_t nb = ((int64_t)a->hidden + MX4_BLOCK - 1) / MX4_BLOCK;

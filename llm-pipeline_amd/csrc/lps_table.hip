@@ -11,7 +11,7 @@ using namespace lps;
 
 namespace {
 
-constexpr int kMaxHidden = 1 << 24;
+constexpr int kMaxPositions = 1 << 30;   // of a gradient: its kernels count a little past them in 32 bits
 
 bool aligned_to(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 size_t elem_bytes(int dtype) { return dtype == LPS_DTYPE_F32 ? 4 : 2; }
@@ -60,7 +60,7 @@ hipError_t launch_quantize(Mx4Params P, hipStream_t s) {
 int check_mx4(const lps_mx4_args* a) {
   if (!a) return LPS_EINVAL;
   if (!dtype_ok(a->dtype)) return LPS_EUNSUPPORTED_DTYPE;
-  if (a->rows < 0 || a->hidden < 1 || a->hidden > kMaxHidden) return LPS_EINVAL;
+  if (a->rows < 0 || a->hidden < 1 || a->hidden > MX4_MAX_HIDDEN) return LPS_EINVAL;
   if (a->rows == 0) return LPS_OK;
   if (!a->x || !a->codes || !a->scales || !aligned_to(a->x, elem_bytes(a->dtype))) return LPS_EINVAL;
   if (!aligned_to(a->codes, 4) || a->codes_stride % 4) return LPS_EINVAL;
@@ -177,7 +177,7 @@ int lps_embedding(const lps_embedding_args* a, void* stream) {
   if (!a) return LPS_EINVAL;
   const bool mx4 = a->dtype == LPS_DTYPE_MX4;
   if ((!mx4 && !dtype_ok(a->dtype)) || !dtype_ok(a->out_dtype)) return LPS_EUNSUPPORTED_DTYPE;
-  if (a->n < 0 || a->vocab < 1 || a->hidden < 1 || a->hidden > kMaxHidden || (a->id_bytes != 4 && a->id_bytes != 8)) return LPS_EINVAL;
+  if (a->n < 0 || a->vocab < 1 || a->hidden < 1 || a->hidden > MX4_MAX_HIDDEN || (a->id_bytes != 4 && a->id_bytes != 8)) return LPS_EINVAL;
   if (a->n == 0) return LPS_OK;
   if (!a->ids || !a->table || !a->out || (mx4 && !a->scales)) return LPS_EINVAL;
   if (!aligned_to(a->ids, a->id_bytes) || !aligned_to(a->table, mx4 ? 4 : elem_bytes(a->dtype)) ||
@@ -212,14 +212,15 @@ int lps_embedding(const lps_embedding_args* a, void* stream) {
 }
 
 size_t lps_embedding_grad_workspace_bytes(int n, int vocab, int hidden) {
-  if (n < 0 || vocab < 1 || hidden < 1 || hidden > kMaxHidden) return 0;
+  if (n < 0 || n > kMaxPositions || vocab < 1 || hidden < 1 || hidden > MX4_MAX_HIDDEN) return 0;
   return eg_workspace(n, vocab, hidden).bytes;
 }
 
 int lps_embedding_grad(const lps_embedding_grad_args* a, void* stream) {
   if (!a) return LPS_EINVAL;
   if (!dtype_ok(a->dtype) || !dtype_ok(a->out_dtype)) return LPS_EUNSUPPORTED_DTYPE;
-  if (a->n < 0 || a->vocab < 1 || a->hidden < 1 || a->hidden > kMaxHidden || (a->id_bytes != 4 && a->id_bytes != 8)) return LPS_EINVAL;
+  if (a->n < 0 || a->n > kMaxPositions || a->vocab < 1 || a->hidden < 1 || a->hidden > MX4_MAX_HIDDEN) return LPS_EINVAL;
+  if (a->id_bytes != 4 && a->id_bytes != 8) return LPS_EINVAL;
   if (a->n == 0 && a->accumulate) return LPS_OK;
   if (!a->out || (a->n > 0 && (!a->ids || !a->grad))) return LPS_EINVAL;
   if (!aligned_to(a->ids, a->id_bytes) || !aligned_to(a->grad, elem_bytes(a->dtype)) ||

@@ -17,7 +17,7 @@ import torch
 
 from . import _device as D
 from . import _lib
-from .vocab_table import Mx4Tensor, _call, _on_gpu, _same_device
+from .vocab_table import Mx4Tensor, _call, _on_gpu, _same_device, _sizes
 
 _pack_mx4 = _lib.packer(_lib.LmHeadMx4Args)
 
@@ -119,6 +119,7 @@ def _lm_head_mx4(hidden, weight, out_dtype, return_stats):
     w, ws = weight.rows()
     ws = _words(ws)
     device, V = w.device, w.shape[0]
+    _sizes(M, V, H)
     out_code = D.code_of(od)
     out = torch.empty((M, V), dtype=od, device=device)
     G = (V + _lib.LMHEAD_BLOCK_COLS - 1) // _lib.LMHEAD_BLOCK_COLS

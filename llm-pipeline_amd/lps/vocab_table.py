@@ -104,6 +104,12 @@ def _call(name: str, args: bytes, device: torch.device) -> None:
         _lib.check(rc, name)
 
 
+def _sizes(*n: int) -> None:
+    """The C ABI counts in 32 bits."""
+    if max(n) > 0x7FFFFFFF:
+        raise ValueError(f"sizes of at most {0x7FFFFFFF} expected; got {max(n)}")
+
+
 def mx4_quantize(x: torch.Tensor) -> Mx4Tensor:
     """``x [..., H]`` (float32, bfloat16 or float16) to microscaled 4-bit floats
     along its last dimension.
@@ -120,6 +126,7 @@ def mx4_quantize(x: torch.Tensor) -> Mx4Tensor:
     xf = _flat_rows(x)
     device = x.device
     rows, hidden = xf.shape
+    _sizes(rows, hidden)
     n = (hidden + 31) // 32
     codes = torch.empty((rows, 16 * n), dtype=torch.uint8, device=device)
     # scale rows on 4-byte lines: the LM head reads four at a time
@@ -144,6 +151,7 @@ def mx4_dequantize(t: Mx4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.T
     code = D.code_of(dtype)
     codes, scales = t.rows()
     rows, device, hidden = codes.shape[0], codes.device, t.hidden
+    _sizes(rows, hidden)
     out = torch.empty((rows, hidden), dtype=dtype, device=device)
     if rows:
         many = rows > 1
@@ -184,6 +192,7 @@ def _embedding(ids: torch.Tensor, table: Union[torch.Tensor, Mx4Tensor], scale: 
     if vocab < 1:
         raise ValueError("the table has no rows")
     device, n = rows.device, flat.shape[0]
+    _sizes(n, vocab, hidden)
     out_code = D.code_of(dtype)
     out = torch.empty((n, hidden), device=device, dtype=dtype)
     if n:
@@ -240,6 +249,7 @@ def embedding_grad(ids: torch.Tensor, grad: torch.Tensor, vocab: int, scale: flo
         raise ValueError(f"vocab must be at least 1; got {vocab}")
     _same_device(ids, grad, "ids and grad")
     device, hidden, n = grad.device, grad.shape[-1], flat.shape[0]
+    _sizes(n, vocab, hidden)
     g = _flat_rows(grad)
     if out is None:
         dtype = dtype or grad.dtype

@@ -56,8 +56,8 @@ def test_embedding_argument_errors(lib, kw, code):  # noqa: F811
 
 @pytest.mark.parametrize("kw,code", [
     (dict(dtype=3), 2), (dict(out_dtype=3), 2), (dict(id_bytes=1), 1), (dict(n=-1), 1), (dict(vocab=0), 1),
-    (dict(hidden=0), 1), (dict(n=0, accumulate=1, out=0), 0), (dict(ids=0), 1), (dict(grad=0), 1), (dict(out=0), 1),
-    (dict(ids=0x1004), 1), (dict(grad=0x2001), 1), (dict(out=0x3002), 1), (dict(grad_stride=63), 1),
+    (dict(n=(1 << 30) + 1), 1), (dict(hidden=0), 1), (dict(n=0, accumulate=1, out=0), 0), (dict(ids=0), 1), (dict(grad=0), 1),
+    (dict(out=0), 1), (dict(ids=0x1004), 1), (dict(grad=0x2001), 1), (dict(out=0x3002), 1), (dict(grad_stride=63), 1),
     (dict(out_stride=63), 1), (dict(workspace=0), 4), (dict(workspace_bytes=16), 4), (dict(workspace=0x4008), 1)])
 def test_embedding_grad_argument_errors(lib, kw, code):  # noqa: F811
     from lps import _lib
@@ -74,8 +74,10 @@ def test_embedding_grad_argument_errors(lib, kw, code):  # noqa: F811
 
 @pytest.mark.parametrize("kw,code", [
     (dict(dtype=0), 2), (dict(out_dtype=3), 2), (dict(rows=-1), 1), (dict(rows=0, x=0), 0), (dict(vocab=0), 1),
-    (dict(hidden=0), 1), (dict(x=0), 1), (dict(w=0), 1), (dict(w_scales=0), 1), (dict(out=0), 1), (dict(x=0x1008), 1),
-    (dict(x_stride=100), 1), (dict(x_stride=96), 1), (dict(w=0x2008), 1), (dict(w_stride=48), 1), (dict(w_stride=72), 1),
+    (dict(hidden=0), 1), (dict(vocab=(1 << 21) + 1), 1), (dict(hidden=(1 << 24) + 1), 1),
+    (dict(x_stride=(1 << 22) + 8), 1), (dict(w_stride=(1 << 23) + 16), 1), (dict(x=0), 1), (dict(w=0), 1),
+    (dict(w_scales=0), 1), (dict(out=0), 1), (dict(x=0x1008), 1), (dict(x_stride=100), 1), (dict(x_stride=96), 1),
+    (dict(w=0x2008), 1), (dict(w_stride=48), 1), (dict(w_stride=72), 1),
     (dict(w_scales=0x3002), 1), (dict(w_scales_stride=6), 1), (dict(w_scales_stride=0), 1), (dict(out_stride=9), 1),
     (dict(dtype=3, x_stride=64), 1),                                                  # 4-bit x without scales
     (dict(dtype=3, x_stride=56, x_scales=0x5000, x_scales_stride=4), 1),
