@@ -3,17 +3,18 @@
 // (added to out[v] when accumulating), summed in fp32 in one fixed order, so a
 // call's result never depends on timing.
 //
-// Up to EG_SMALL positions, one launch: grad_small_kernel.  More, three:
+// Up to EG_SMALL positions grad_small_kernel, after grad_zero_kernel where there are
+// many zeros to write.  More, three launches:
 // 1. grad_sort_kernel groups the positions by id.  Workgroup w of G takes the
 //    ids with id % G == w (neighbouring frequent ids land apart); it reads all
 //    ids, counts its own and those of the workgroups before it (its place in
 //    the order, so no workgroup waits for another), and places its positions by
-//    id, in their own order.
+//    id, in their own order.  For a new gradient more workgroups of the launch write
+//    zeros to all rows meanwhile.
 // 2. grad_tiles_kernel cuts that order into tiles of S positions (a frequent id
 //    costs no one workgroup more than another) and adds the gradient rows of
 //    each run of one id.  A run inside a tile is written at once; a run's part
-//    in a tile that it enters or leaves goes to that tile's partial rows.  For a
-//    new gradient more workgroups of the launch zero the rows without a token.
+//    in a tile that it enters or leaves goes to that tile's partial rows.
 // 3. grad_join_kernel adds the partial rows of each run that crosses tiles.
 #pragma once
 
@@ -26,11 +27,12 @@ namespace lps {
 constexpr int EG_NT = 1024;         // threads of the sort
 constexpr int EG_NW = EG_NT / 64;
 constexpr int EG_OWN = 1024;        // ids a workgroup of the sort can own
-constexpr int EG_LIST = 4096;       // positions it keeps in LDS
+constexpr int EG_LIST = 3968;       // positions it keeps in LDS: as many as leave room for two workgroups a CU
+constexpr int EG_POS_BITS = 22;     // .. whose ids take the other 10
 constexpr int EG_SMAX = 1024;       // positions of a tile, at most
-constexpr int EG_FILL = 8192;       // bytes of rows that a zeroing workgroup looks at, or one row
+constexpr int EG_FILL = 1 << 21;    // workgroups that write zeros: at most
 constexpr int EG_JOIN = 8;          // tiles a joining workgroup looks at
-constexpr int EG_SMALL = 2048;      // positions of the one-launch form
+constexpr int EG_SMALL = 768;       // positions of the form without a sort
 
 struct EmbGradParams {
   const void* ids;
@@ -42,37 +44,102 @@ struct EmbGradParams {
   int accumulate;
   int lg_groups;         // log2 G
   int S, tiles, slices;  // positions of a tile; tiles; workgroups on a tile
-  int fill_rows;         // rows of a zeroing workgroup
+  int zero;              // grad_small_kernel: rows without a token become zero
+  int fill_lines;        // 16-byte lines that a row can lie in
   // workspace
   int* count;            // [1] positions with a valid id
   int* sid;              // [n] ids in the order
   int* spos;             // [n] positions in the order
   int* tmp_id;           // [n] lists that outgrow LDS
   int* tmp_pos;          // [n]
-  uint8_t* touched;      // [vocab], new gradients
   float* part;           // [2 tiles, part_stride]: runs entering, runs leaving
   int64_t part_stride;
 };
 
+// Zeros to all rows of a new gradient, those with a token among them: they are
+// written again by a later launch, and leaving them out costs more (1.2 GB 250 us).
+// Chunk c is 256 of the 16-byte lines that the rows lie in, one of them a thread's.
+template <int ODT>
+__device__ __forceinline__ void grad_zero_chunk(const EmbGradParams& P, int64_t c, int t) {
+  constexpr int ES = ElemBytes<ODT>::value;
+  const int64_t first = c * 256;
+  const uint32_t lines = (uint32_t)P.fill_lines;
+  int64_t row;
+  uint32_t q;
+  if (first >> 32) {
+    row = first / lines;
+    q = (uint32_t)(first - row * lines);
+  } else {
+    const uint32_t f = (uint32_t)first;
+    row = f / lines;
+    q = f % lines;
+  }
+  q += t;
+  row += q / lines;
+  q %= lines;
+  if (row >= P.vocab) return;
+  // the line whole, or the row's part of it
+  const int64_t bytes = (int64_t)P.hidden * ES;
+  const uintptr_t p = reinterpret_cast<uintptr_t>(P.out) + row * P.out_stride * ES;
+  const uintptr_t line = (p & ~(uintptr_t)15) + (uintptr_t)q * 16;
+  if (line >= p && line + 16 <= p + bytes) {
+    *reinterpret_cast<u32x4*>(line) = u32x4{};
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; e += ES) {
+      if (line + e >= p && line + e < p + bytes) {
+        if constexpr (ES == 4) *reinterpret_cast<uint32_t*>(line + e) = 0;
+        else *reinterpret_cast<uint16_t*>(line + e) = 0;
+      }
+    }
+  }
+}
+// Workgroup wg of wgs, NT threads: NT / 256 chunks at a time.  Memory takes zeros best
+// in its order, and where chunks of 4 KB go to the XCDs in turn, as workgroups do:
+// 1.2 GB in workgroups of 256 take 181 us with a chunk each and 195 with two
+// neighbouring ones; beside the sort, in workgroups of 1024, 195 with every eighth
+// chunk, 217 with four neighbouring ones and 250 in a loop of 512 workgroups.
+template <int ODT, int NT>
+__device__ __forceinline__ void grad_zero(const EmbGradParams& P, int wg, int wgs) {
+  const int64_t chunks = ((int64_t)P.vocab * P.fill_lines + 255) >> 8;
+  constexpr int C = NT / 256;
+  const int part = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 8);
+  for (int64_t w = wg; (w >> 3) * (8 * C) < chunks; w += wgs)
+    grad_zero_chunk<ODT>(P, (w >> 3) * (8 * C) + 8 * part + (w & 7), (int)threadIdx.x & 255);
+}
+template <int ODT>
+__global__ __launch_bounds__(256) void grad_zero_kernel(EmbGradParams P) {
+  grad_zero<ODT, 256>(P, (int)blockIdx.x, (int)gridDim.x);
+}
+
 // What bounds the sort is latency: every workgroup reads all ids (from its L2), lists
 // its own in order (waves take runs of positions), and cuts the list into a run per
 // wave: counts by id and wave, one scan over both, and each wave places its run.
-// 8192 ids 13 us, 32768 19 us (with one wave that places the whole list 17 and 27).
-__global__ __launch_bounds__(EG_NT) void grad_sort_kernel(EmbGradParams P) {
+// 8192 ids 9 us, 32768 15.5 us (with one wave that places the whole list 17 and 27).
+// 64 VGPRs and half of a CU's LDS, so that a workgroup that writes zeros runs beside it.
+template <int ODT>
+__global__ __launch_bounds__(EG_NT, 8) void grad_sort_kernel(EmbGradParams P) {
   __shared__ uint32_t count[EG_NW][EG_OWN];        // positions of an id in a wave's run; then their next place
-  __shared__ int list_id[EG_LIST], list_pos[EG_LIST];
+  __shared__ uint32_t list[EG_LIST];
   __shared__ int wcnt[EG_NW], wless[EG_NW], wall[EG_NW];
   __shared__ uint32_t wsum[EG_NW];
   const int tid = (int)threadIdx.x, wv = tid >> 6, l = tid & 63;
   const int w = (int)blockIdx.x, lg = P.lg_groups, mask = (1 << lg) - 1;
+  if (w > mask) {
+    grad_zero<ODT, EG_NT>(P, w - mask - 1, (int)gridDim.x - mask - 1);
+    return;
+  }
   const int own = w < P.vocab ? (P.vocab - 1 - w) / (mask + 1) + 1 : 0;   // ids w, w + G, ..
   // each wave takes a run of positions, 64 U at a time
   const int per = ((P.n + EG_NW - 1) / EG_NW + 63) & ~63;
   const int64_t a64 = (int64_t)wv * per;
   const int a = a64 < P.n ? (int)a64 : P.n, b = P.n - a < per ? P.n : a + per;
-  constexpr int U = 8, R = 4;                      // (R batches are kept for the second pass)
-  int kept[R][U];                                  // ids (-1 without one)
-  auto fetch = [&](int i0, int (&id)[U]) {
+  static_assert(EG_OWN == 1 << (32 - EG_POS_BITS), "an id and a position to a word");
+  constexpr int U = 4, R = 8;
+  constexpr int NONE = 0xFFFF;                     // an id of another workgroup's
+  uint32_t kept[R][U / 2];                         // R batches for the second pass: ids' places among the own ones
+  int cnt = 0, less = 0, all = 0;                  // this lane's
+  auto fetch = [&](int i0, int (&place)[U], bool tally) {
     int64_t v[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -80,29 +147,30 @@ __global__ __launch_bounds__(EG_NT) void grad_sort_kernel(EmbGradParams P) {
       v[u] = i < b ? load_id(P.ids, P.id_bytes, i) : -1;
     }
 #pragma unroll
-    for (int u = 0; u < U; u++) id[u] = v[u] >= 0 && v[u] < P.vocab ? (int)v[u] : -1;
-  };
-#pragma unroll
-  for (int r = 0; r < R; r++)
-    if ((int64_t)a + 64 * U * r < b) fetch(a + 64 * U * r, kept[r]);
-  for (int k = l; k < own; k += 64) count[wv][k] = 0;
-  int cnt = 0, less = 0, all = 0;                  // this lane's
-  auto tally = [&](const int (&id)[U]) {
-#pragma unroll
     for (int u = 0; u < U; u++) {
-      const bool valid = id[u] >= 0;
-      cnt += valid && (id[u] & mask) == w;
-      less += valid && (id[u] & mask) < w;
-      all += valid;
+      const bool valid = v[u] >= 0 && v[u] < P.vocab;
+      const int g = (int)v[u] & mask;
+      place[u] = valid && g == w ? (int)v[u] >> lg : NONE;
+      if (tally) {
+        cnt += valid && g == w;
+        less += valid && g < w;
+        all += valid;
+      }
     }
   };
+  for (int k = l; k < own; k += 64) count[wv][k] = 0;
 #pragma unroll
-  for (int r = 0; r < R; r++)
-    if ((int64_t)a + 64 * U * r < b) tally(kept[r]);
+  for (int r = 0; r < R; r++) {
+    if ((int64_t)a + 64 * U * r < b) {
+      int place[U];
+      fetch(a + 64 * U * r, place, true);
+#pragma unroll
+      for (int u = 0; u < U; u += 2) kept[r][u / 2] = (uint32_t)place[u] | (uint32_t)place[u + 1] << 16;
+    }
+  }
   for (int64_t i0 = (int64_t)a + 64 * U * R; i0 < b; i0 += 64 * U) {
-    int id[U];
-    fetch((int)i0, id);
-    tally(id);
+    int place[U];
+    fetch((int)i0, place, true);
   }
   cnt = lps::wsum(cnt);
   less = lps::wsum(less);
@@ -118,47 +186,49 @@ __global__ __launch_bounds__(EG_NT) void grad_sort_kernel(EmbGradParams P) {
   }
   if (w == 0 && tid == 0) *P.count = every;
   // the workgroup's positions in their own order
-  const bool in_lds = total <= EG_LIST;
+  const bool in_lds = total <= EG_LIST && P.n <= 1 << EG_POS_BITS;
   int* const gid = P.tmp_id + start;
   int* const gpos = P.tmp_pos + start;
-  auto place = [&](int i0, const int (&id)[U]) {
+  auto append = [&](int i0, const int (&place)[U]) {
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const bool mine = id[u] >= 0 && (id[u] & mask) == w;
+      const bool mine = place[u] != NONE;
       const uint64_t m = wballot(mine);
       if (mine) {
         const int k = at + (int)lanes_below(m), i = i0 + 64 * u + l;
-        if (in_lds) { list_id[k] = id[u] >> lg; list_pos[k] = i; }
-        else { gid[k] = id[u] >> lg; gpos[k] = i; }
+        if (in_lds) list[k] = (uint32_t)place[u] << EG_POS_BITS | (uint32_t)i;
+        else { gid[k] = place[u]; gpos[k] = i; }
       }
       at += __builtin_popcountll(m);
     }
   };
 #pragma unroll
-  for (int r = 0; r < R; r++)
-    if ((int64_t)a + 64 * U * r < b) place(a + 64 * U * r, kept[r]);
+  for (int r = 0; r < R; r++) {
+    if ((int64_t)a + 64 * U * r < b) {
+      int place[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) place[u] = (int)(kept[r][u / 2] >> (16 * (u & 1)) & 0xFFFF);
+      append(a + 64 * U * r, place);
+    }
+  }
   for (int64_t i0 = (int64_t)a + 64 * U * R; i0 < b; i0 += 64 * U) {
-    int id[U];
-    fetch((int)i0, id);
-    place((int)i0, id);
+    int place[U];
+    fetch((int)i0, place, false);
+    append((int)i0, place);
   }
   __syncthreads();
   // this wave's run of the list
   const int run = ((total + EG_NW - 1) / EG_NW + 63) & ~63;
   const int k0 = wv * run < total ? wv * run : total, k1 = total - k0 < run ? total : k0 + run;
-  for (int k = k0 + l; k < k1; k += 64) atomicAdd(&count[wv][in_lds ? list_id[k] : gid[k]], 1u);
+  for (int k = k0 + l; k < k1; k += 64) atomicAdd(&count[wv][in_lds ? (int)(list[k] >> EG_POS_BITS) : gid[k]], 1u);
   __syncthreads();
   {
     // a thread's id: its positions over the waves, its place over the ids
-    uint32_t c[EG_NW], s = 0;
+    uint32_t s = 0;
     if (tid < own) {
 #pragma unroll
-      for (int k = 0; k < EG_NW; k++) {
-        c[k] = count[k][tid];
-        s += c[k];
-      }
+      for (int k = 0; k < EG_NW; k++) s += count[k][tid];
     }
-    if (P.touched && tid < own) P.touched[w + ((int64_t)tid << lg)] = s != 0;
     const uint32_t incl = wscan_incl(s);
     if (l == 63) wsum[wv] = incl;
     __syncthreads();
@@ -167,8 +237,9 @@ __global__ __launch_bounds__(EG_NT) void grad_sort_kernel(EmbGradParams P) {
     if (tid < own) {
 #pragma unroll
       for (int k = 0; k < EG_NW; k++) {
+        const uint32_t c = count[k][tid];
         count[k][tid] = p;
-        p += c[k];
+        p += c;
       }
     }
   }
@@ -179,7 +250,12 @@ __global__ __launch_bounds__(EG_NT) void grad_sort_kernel(EmbGradParams P) {
   for (int q = k0; q < k1; q += 64) {
     const int k = q + l;
     const bool on = k < k1;
-    const int id = on ? (in_lds ? list_id[k] : gid[k]) : 0, pos = on ? (in_lds ? list_pos[k] : gpos[k]) : 0;
+    int id = 0, pos = 0;
+    if (on) {
+      const uint32_t x = in_lds ? list[k] : 0;
+      id = in_lds ? (int)(x >> EG_POS_BITS) : gid[k];
+      pos = in_lds ? (int)(x & ((1u << EG_POS_BITS) - 1)) : gpos[k];
+    }
     uint64_t same = wballot(on);
     for (int i = 0; i < bits; i++) {
       const bool one = (id >> i) & 1;
@@ -217,21 +293,6 @@ template <int GDT, int ODT>
 __global__ __launch_bounds__(256) void grad_tiles_kernel(EmbGradParams P) {
   __shared__ int s_id[EG_SMAX + 2], s_pos[EG_SMAX];
   const int tid = (int)threadIdx.x;
-  const int64_t work = (int64_t)P.tiles * P.slices;
-  if (blockIdx.x >= work) {
-    // rows without a token: as many neighbouring ones as EG_FILL bytes hold, so that
-    // the launch writes memory in its order (1.2 GB in rows of 8 KB: 194 us at a row
-    // to a workgroup, 215 at 16, 231 at 149)
-    const int64_t r0 = ((int64_t)blockIdx.x - work) * P.fill_rows;
-    const float zero[8] = {};
-    const int pieces = (P.hidden + 7) >> 3;
-    for (int i = tid; i < P.fill_rows * pieces; i += 256) {
-      const int64_t row = r0 + i / pieces;
-      if (row < P.vocab && !P.touched[row])
-        store_piece<ODT>(static_cast<char*>(P.out) + row * P.out_stride * ElemBytes<ODT>::value, 8 * (i % pieces), P.hidden, zero);
-    }
-    return;
-  }
   const int t = (int)(blockIdx.x / (unsigned)P.slices), sl = (int)(blockIdx.x % (unsigned)P.slices);
   const int nv = *P.count;
   const int64_t base64 = (int64_t)t * P.S;
@@ -464,7 +525,7 @@ __global__ __launch_bounds__(256) void grad_small_kernel(EmbGradParams P) {
       add(x, j, 1, acc);
       grad_write<ODT>(P, (x << lg) + w, e0, acc);
     }
-    if (!P.accumulate) {
+    if (P.zero) {
       const float zero[8] = {};
       for (int x = k; x < own; x += 8)
         if (times[x] == 0)

@@ -70,7 +70,7 @@ int check_mx4(const lps_mx4_args* a) {
 }
 
 struct EgWs {
-  size_t count, sid, spos, tmp_id, tmp_pos, touched, part, bytes;
+  size_t count, sid, spos, tmp_id, tmp_pos, part, bytes;
 };
 // Positions of a tile: about 2048 tiles, so that a frequent token's rows spread
 // over the card and a tile's loads are in flight together.
@@ -79,7 +79,9 @@ int eg_tile(int n) {
   while (s < EG_SMAX && (int64_t)s * 2048 < n) s *= 2;
   return s;
 }
-// One launch, without a workspace: few positions, and ids that 4096 workgroups can own.
+// Without a sort and a workspace: few positions (a new fp32 gradient of 1000 to 4000 rows: 517
+// positions about 12 us against 17, 1000 22 to 35 against 17 to 28, even at 768), and
+// ids that 4096 workgroups can own.
 bool eg_small(int n, int vocab) { return n <= EG_SMALL && vocab <= 4096 * EG_OWN; }
 EgWs eg_workspace(int n, int vocab, int hidden) {
   EgWs w{};
@@ -97,18 +99,31 @@ EgWs eg_workspace(int n, int vocab, int hidden) {
   w.spos = take((size_t)n * 4);
   w.tmp_id = take((size_t)n * 4);
   w.tmp_pos = take((size_t)n * 4);
-  w.touched = take((size_t)vocab);
   w.part = take(tiles * 2 * (((size_t)hidden + 7) / 8 * 8) * 4);
   w.bytes = at;
   return w;
 }
 
+// Workgroups of `threads` that zero all rows: 16 bytes a thread, whole eights, up to
+// EG_FILL (a launch has fewer than 2^32 threads).
+unsigned fill_wgs(const EmbGradParams& P, int threads) {
+  const int64_t eights = ((int64_t)P.vocab * P.fill_lines + 8 * threads - 1) / (8 * threads);
+  return eights < EG_FILL / 8 ? 8 * (unsigned)eights : (unsigned)EG_FILL;
+}
+
 template <int GDT, int ODT>
 hipError_t launch_grad(EmbGradParams P, hipStream_t s) {
+  const int64_t bytes = P.accumulate ? 0 : (int64_t)P.vocab * P.hidden * ElemBytes<ODT>::value;
   if (eg_small(P.n, P.vocab)) {
+    // more zeros than the L2s hold: in a launch before
+    P.zero = !P.accumulate && bytes <= MX4_STREAM;
+    if (bytes > MX4_STREAM) {
+      hipLaunchKernelGGL((grad_zero_kernel<ODT>), dim3(fill_wgs(P, 256)), dim3(256), 0, s, P);
+    }
+    if (P.n == 0 && !P.zero) return hipGetLastError();
     // about eight positions and 64 thousand values of zeros a workgroup, up to one on
     // each CU; more where it would own more ids than it can count
-    const int64_t values = P.accumulate ? 0 : (int64_t)P.vocab * (P.hidden < 256 ? P.hidden : 256);
+    const int64_t values = P.zero ? (int64_t)P.vocab * (P.hidden < 256 ? P.hidden : 256) : 0;
     int lg = 4;
     while (lg < 8 && ((8 << lg) < P.n || (values >> lg) > 65536)) lg++;
     while (((int64_t)P.vocab + (1 << lg) - 1) >> lg > EG_OWN) lg++;
@@ -116,9 +131,8 @@ hipError_t launch_grad(EmbGradParams P, hipStream_t s) {
     hipLaunchKernelGGL((grad_small_kernel<GDT, ODT>), dim3(1u << lg, (unsigned)((P.hidden + 255) / 256)), dim3(256), 0, s, P);
     return hipGetLastError();
   }
-  hipLaunchKernelGGL(grad_sort_kernel, dim3(1u << P.lg_groups), dim3(EG_NT), 0, s, P);
-  const int64_t fill = P.touched ? ((int64_t)P.vocab + P.fill_rows - 1) / P.fill_rows : 0;
-  hipLaunchKernelGGL((grad_tiles_kernel<GDT, ODT>), dim3((unsigned)((int64_t)P.tiles * P.slices + fill)), dim3(256), 0, s, P);
+  hipLaunchKernelGGL((grad_sort_kernel<ODT>), dim3((1u << P.lg_groups) + (P.accumulate ? 0 : fill_wgs(P, EG_NT))), dim3(EG_NT), 0, s, P);
+  hipLaunchKernelGGL((grad_tiles_kernel<GDT, ODT>), dim3((unsigned)((int64_t)P.tiles * P.slices)), dim3(256), 0, s, P);
   if (P.tiles > 1)
     hipLaunchKernelGGL((grad_join_kernel<ODT>), dim3((unsigned)((P.tiles - 1 + EG_JOIN - 1) / EG_JOIN), (unsigned)((P.hidden + 255) / 256)), dim3(256), 0, s, P);
   return hipGetLastError();
@@ -253,15 +267,15 @@ int lps_embedding_grad(const lps_embedding_grad_args* a, void* stream) {
   P.tiles = (int)(((int64_t)a->n + P.S - 1) / P.S);
   P.slices = (a->hidden + 2047) / 2048;
   const int64_t row_bytes = (int64_t)a->hidden * elem_bytes(a->out_dtype);
-  P.fill_rows = row_bytes < EG_FILL ? (int)(EG_FILL / row_bytes) : 1;
-  const int64_t grid = (int64_t)P.tiles * P.slices + ((int64_t)a->vocab + P.fill_rows - 1) / P.fill_rows;
-  if (grid > 0x7FFFFFFF || (a->hidden + 255) / 256 > 65535) return LPS_EINVAL;
+  P.zero = !P.accumulate;
+  P.fill_lines = aligned_to(a->out, 16) && P.out_stride * elem_bytes(a->out_dtype) % 16 == 0
+                     ? (int)((row_bytes + 15) / 16) : (int)((row_bytes + 14) / 16) + 1;
+  if ((int64_t)P.tiles * P.slices > 0x7FFFFFFF || (a->hidden + 255) / 256 > 65535) return LPS_EINVAL;
   P.count = reinterpret_cast<int*>(ws + w.count);
   P.sid = reinterpret_cast<int*>(ws + w.sid);
   P.spos = reinterpret_cast<int*>(ws + w.spos);
   P.tmp_id = reinterpret_cast<int*>(ws + w.tmp_id);
   P.tmp_pos = reinterpret_cast<int*>(ws + w.tmp_pos);
-  P.touched = P.accumulate ? nullptr : reinterpret_cast<uint8_t*>(ws + w.touched);
   P.part = reinterpret_cast<float*>(ws + w.part);
   P.part_stride = ((int64_t)a->hidden + 7) / 8 * 8;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);

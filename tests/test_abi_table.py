@@ -98,8 +98,8 @@ def test_lm_head_mx4_argument_errors(lib, kw, code):  # noqa: F811
 def test_workspace_bytes(lib):  # noqa: F811
     f = lib.lps_embedding_grad_workspace_bytes
     assert f(-1, 10, 10) == f(3, 0, 10) == f(3, 10, 0) == 0
-    assert f(0, 10, 10) == f(2048, 151936, 4096) == 0             # one launch, no workspace
-    assert 0 < f(2049, 10, 10) <= f(2049, 10, 1000) <= f(100000, 10, 1000)
+    assert f(0, 10, 10) == f(768, 151936, 4096) == 0              # few positions: no workspace
+    assert 0 < f(769, 10, 10) <= f(2049, 10, 1000) <= f(100000, 10, 1000)
     assert f(5, 1 << 30, 8) > 0
 
 

@@ -293,3 +293,21 @@ def test_refusals(dev):
         lps.embedding_grad(ids, x[:3], 4, out=x, dtype=torch.bfloat16)
     with pytest.raises(ValueError):
         lps.embedding_grad(ids, x[:3], 4, out=x.clone().requires_grad_())
+
+
+@pytest.mark.parametrize("n,vocab,hidden,dtype", [(0, 9001, 1023, torch.float32), (3, 70000, 131, torch.float32),
+                                                  (900, 30001, 601, torch.bfloat16), (1025, 40000, 517, torch.float16),
+                                                  (1500, 1 << 20, 4104, torch.float32), (2, 1 << 20, 4104, torch.float32)])
+def test_gradient_writes_every_zero(dev, n, vocab, hidden, dtype):
+    """Outputs past the L2s, two of them past 16 GB: rows without a token are zeros
+    whatever the memory held, the last id's row is its gradient."""
+    torch.full((vocab, hidden), 3.0, dtype=dtype, device=dev)       # freed at once: the same memory
+    g = torch.Generator().manual_seed(n)
+    ids = torch.randint(0, vocab, (n,), generator=g)
+    ids[n // 2:] = vocab - 1
+    grad = torch.ones((n, hidden), dtype=dtype)
+    got = lps.embedding_grad(ids.to(dev), grad.to(dev), vocab)
+    times = torch.bincount(ids, minlength=vocab)
+    assert bool((got[times.nonzero()[:, 0].to(dev)].cpu() == times[times > 0, None]).all())
+    got[times.nonzero()[:, 0].to(dev)] = 0
+    assert int(torch.count_nonzero(got)) == 0
