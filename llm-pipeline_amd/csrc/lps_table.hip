@@ -27,7 +27,7 @@ int lg_threads_per_row(int pieces) {
 
 template <int TDT, int ODT>
 hipError_t launch_gather(GatherParams P, hipStream_t s) {
-  const int pieces = (P.hidden + 7) / 8;
+  const int pieces = (P.hidden + GATHER_VALUES<ODT> - 1) / GATHER_VALUES<ODT>;
   P.lg_tpr = lg_threads_per_row(pieces);
   const int64_t wgs = (P.n + (256 >> P.lg_tpr) - 1) >> (8 - P.lg_tpr);
   // few rows: a long row over several workgroups
