@@ -107,7 +107,7 @@ EgWs eg_workspace(int n, int vocab, int hidden) {
 // Workgroups of `threads` that zero all rows: 16 bytes a thread, whole eights, up to
 // EG_FILL (a launch has fewer than 2^32 threads).
 unsigned fill_wgs(const EmbGradParams& P, int threads) {
-  const int64_t eights = ((int64_t)P.vocab * P.fill_lines + 8 * threads - 1) / (8 * threads);
+  const int64_t eights = (P.fill_rows * P.fill_lines + 8 * threads - 1) / (8 * threads);
   return eights < EG_FILL / 8 ? 8 * (unsigned)eights : (unsigned)EG_FILL;
 }
 
@@ -268,8 +268,11 @@ int lps_embedding_grad(const lps_embedding_grad_args* a, void* stream) {
   P.slices = (a->hidden + 2047) / 2048;
   const int64_t row_bytes = (int64_t)a->hidden * elem_bytes(a->out_dtype);
   P.zero = !P.accumulate;
-  P.fill_lines = aligned_to(a->out, 16) && P.out_stride * elem_bytes(a->out_dtype) % 16 == 0
-                     ? (int)((row_bytes + 15) / 16) : (int)((row_bytes + 14) / 16) + 1;
+  const bool whole = P.out_stride == a->hidden;
+  P.fill_rows = whole ? 1 : a->vocab;
+  P.fill_bytes = whole ? a->vocab * row_bytes : row_bytes;
+  P.fill_lines = aligned_to(a->out, 16) && P.out_stride * elem_bytes(a->out_dtype) % 16 == 0 ? (P.fill_bytes + 15) / 16
+                                                                                            : (P.fill_bytes + 14) / 16 + 1;
   if ((int64_t)P.tiles * P.slices > 0x7FFFFFFF || (a->hidden + 255) / 256 > 65535) return LPS_EINVAL;
   P.count = reinterpret_cast<int*>(ws + w.count);
   P.sid = reinterpret_cast<int*>(ws + w.sid);

@@ -311,3 +311,25 @@ def test_gradient_writes_every_zero(dev, n, vocab, hidden, dtype):
     assert bool((got[times.nonzero()[:, 0].to(dev)].cpu() == times[times > 0, None]).all())
     got[times.nonzero()[:, 0].to(dev)] = 0
     assert int(torch.count_nonzero(got)) == 0
+
+
+@pytest.mark.parametrize("n", [3, 1500])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradient_into_rows_of_a_wider_buffer(dev, n, dtype):
+    """The C entry point's new gradient with a row stride: zeros in its rows, nothing beside them."""
+    import ctypes
+    from lps import _lib
+    lib, vocab, hidden = _lib.load(), 9000, 1051
+    buf = torch.full((vocab, 1061), 7.0, dtype=dtype, device=dev)
+    ids = torch.arange(n, device=dev) % 5
+    grad = torch.ones((n, hidden), dtype=dtype, device=dev)
+    bytes_ = lib.lps_embedding_grad_workspace_bytes(n, vocab, hidden)
+    ws = torch.empty((max(bytes_, 16),), dtype=torch.uint8, device=dev)
+    code = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]
+    a = _lib.EmbeddingGradArgs(ids.data_ptr(), grad.data_ptr(), buf[:, 3:].data_ptr(), 8, code, code, n, vocab, hidden,
+                               hidden, 1061, 1.0, 0, ws.data_ptr(), bytes_)
+    assert lib.lps_embedding_grad(ctypes.byref(a), torch.cuda.current_stream().cuda_stream) == 0
+    times = torch.bincount(ids, minlength=5).to(dtype)
+    assert bool((buf[:5, 3:3 + hidden] == times[:, None]).all())
+    assert int(torch.count_nonzero(buf[5:, 3:3 + hidden])) == 0
+    assert bool((buf[:, :3] == 7).all()) and bool((buf[:, 3 + hidden:] == 7).all())
