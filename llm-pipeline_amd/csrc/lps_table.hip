@@ -82,7 +82,7 @@ int eg_tile(int n) {
 // Without a sort and a workspace: few positions (a new fp32 gradient of 1000 to 4000 rows: 517
 // positions about 12 us against 17, 1000 22 to 35 against 17 to 28, even at 768), and
 // ids that 4096 workgroups can own.
-bool eg_small(int n, int vocab) { return n <= EG_SMALL && vocab <= 4096 * EG_OWN; }
+bool eg_small(int n, int vocab) { return n == 0 || (n <= EG_SMALL && vocab <= 4096 * EG_OWN); }
 EgWs eg_workspace(int n, int vocab, int hidden) {
   EgWs w{};
   size_t at = 0;
@@ -115,12 +115,12 @@ template <int GDT, int ODT>
 hipError_t launch_grad(EmbGradParams P, hipStream_t s) {
   const int64_t bytes = P.accumulate ? 0 : (int64_t)P.vocab * P.hidden * ElemBytes<ODT>::value;
   if (eg_small(P.n, P.vocab)) {
-    // more zeros than the L2s hold: in a launch before
-    P.zero = !P.accumulate && bytes <= MX4_STREAM;
-    if (bytes > MX4_STREAM) {
+    // more zeros than the L2s hold: in a launch before; of no positions the zeros are all
+    P.zero = !P.accumulate && bytes <= MX4_STREAM && P.n > 0;
+    if (bytes > 0 && !P.zero) {
       hipLaunchKernelGGL((grad_zero_kernel<ODT>), dim3(fill_wgs(P, 256)), dim3(256), 0, s, P);
     }
-    if (P.n == 0 && !P.zero) return hipGetLastError();
+    if (P.n == 0) return hipGetLastError();
     // about eight positions and 64 thousand values of zeros a workgroup, up to one on
     // each CU; more where it would own more ids than it can count
     const int64_t values = P.zero ? (int64_t)P.vocab * (P.hidden < 256 ? P.hidden : 256) : 0;

@@ -167,6 +167,34 @@ int head(const int32_t* h, FILE* f, FILE* o) {
   return 0;
 }
 
+// {5, entry (1 to 4 as above, 5 dequantises), dtype, out_dtype, rows or n, vocab, hidden, accumulate}: the
+// entry point's launches alone (LPS_EMU_LAUNCHES), over addresses that nothing is at;
+// its return code.
+int launches(const int32_t* h, FILE* o) {
+  if (!getenv("LPS_EMU_LAUNCHES")) return 2;
+  char* const at = reinterpret_cast<char*>((uintptr_t)1 << 40);
+  const int dtype = h[2], out_dtype = h[3], n = h[4], V = h[5], H = h[6], nb = (H + 31) / 32;
+  int32_t rc = -1;
+  if (h[1] == 1 || h[1] == 5) {
+    lps_mx4_args a{at, at, at, dtype, n, H, H, 16 * nb, nb};
+    rc = h[1] == 1 ? lps_mx4_quantize(&a, nullptr) : lps_mx4_dequantize(&a, nullptr);
+  } else if (h[1] == 2) {
+    lps_embedding_args a{at, at, at, at, 8, dtype, out_dtype, n, V, H, dtype == 3 ? 16 * nb : H, nb, H, 1.0f};
+    rc = lps_embedding(&a, nullptr);
+  } else if (h[1] == 3) {
+    lps_embedding_grad_args a{at, at, at, 8, dtype, out_dtype, n, V, H, H, H, 1.0f, h[7], at,
+                              lps_embedding_grad_workspace_bytes(n, V, H)};
+    rc = lps_embedding_grad(&a, nullptr);
+  } else if (h[1] == 4) {
+    const int ss = (nb + 3) & ~3;
+    lps_lm_head_mx4_args a{at, at, at, at, at, nullptr, dtype, out_dtype, n, V, H,
+                           dtype == 3 ? 16 * nb : (H + 7) & ~7, ss, 16 * nb, ss, V};
+    rc = lps_lm_head_mx4(&a, nullptr);
+  }
+  fwrite(&rc, 4, 1, o);
+  return 0;
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
@@ -176,7 +204,7 @@ int main(int argc, char** argv) {
   if (!f || !o) return 2;
   int32_t h[16];
   if (fread(h, 4, 16, f) != 16) return 2;
-  const int rc = h[0] == 1 ? quantise(h, f, o) : h[0] == 2 ? lookup(h, f, o) : h[0] == 3 ? gradient(h, f, o) : h[0] == 4 ? head(h, f, o) : 2;
+  const int rc = h[0] == 1 ? quantise(h, f, o) : h[0] == 2 ? lookup(h, f, o) : h[0] == 3 ? gradient(h, f, o) : h[0] == 4 ? head(h, f, o) : h[0] == 5 ? launches(h, o) : 2;
   fclose(f);
   fclose(o);
   return rc;

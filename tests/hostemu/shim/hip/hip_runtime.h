@@ -48,7 +48,7 @@
 
 typedef int hipError_t;
 typedef void* hipStream_t;
-enum { hipSuccess = 0, hipErrorNotInitialized = 3, hipErrorInvalidValue = 1 };
+enum { hipSuccess = 0, hipErrorNotInitialized = 3, hipErrorInvalidValue = 1, hipErrorInvalidConfiguration = 9 };
 enum { hipDeviceAttributeMultiprocessorCount = 0 };
 enum { hipMemcpyDeviceToHost = 2 };
 
@@ -182,7 +182,34 @@ inline T from_bits(uint64_t b) {
   return v;
 }
 
-inline void launch(dim3 grid, dim3 block, std::function<void()> body) {
+// A launch as the runtime takes it: no empty dimension, at most 1024 threads a
+// workgroup, fewer than 2^32 threads along x, at most 65536 workgroups along y
+// and z.  One that is not leaves an error for hipGetLastError and does not run.
+inline hipError_t g_error = hipSuccess;
+inline bool launch_fits(dim3 g, dim3 b) {
+  return g.x && g.y && g.z && b.x && b.y && b.z && (uint64_t)b.x * b.y * b.z <= 1024 &&
+         (uint64_t)g.x * b.x <= 0xFFFFFFFFull && g.y <= 65536 && g.z <= 65536;
+}
+// With LPS_EMU_LAUNCHES=FILE a process's launches are listed there, a line each
+// (whether it is taken, grid, block, the function that launches), and not run.
+// With LPS_EMU_FAIL=K its launch K (0, 1, ..) is not taken.
+inline int g_launches = 0;
+inline bool launch_taken(dim3 g, dim3 b, const char* from) {
+  static const char* const fail = getenv("LPS_EMU_FAIL");
+  static const char* const path = getenv("LPS_EMU_LAUNCHES");
+  static FILE* const list = path ? fopen(path, "w") : nullptr;
+  const bool taken = launch_fits(g, b) && !(fail && g_launches == atoi(fail));
+  g_launches++;
+  if (!taken) g_error = hipErrorInvalidConfiguration;
+  if (list) {
+    fprintf(list, "%d %u %u %u %u %s\n", (int)taken, g.x, g.y, g.z, b.x * b.y * b.z, from);
+    fflush(list);
+  }
+  return taken && !list;
+}
+
+inline void launch(dim3 grid, dim3 block, const char* from, std::function<void()> body) {
+  if (!launch_taken(grid, block, from)) return;
   watchdog_start();
   g_launching.store(1);
   g_bdim = Tid{block.x, block.y, block.z};
@@ -268,8 +295,12 @@ inline int dpp_src(int l, int ctrl) {
 
 inline void __syncthreads() { lps_emu::t_blk->bar.wait(); }
 
-#define hipLaunchKernelGGL(K, G, B, SHM, STREAM, ...) ::lps_emu::launch(dim3(G), dim3(B), [=]() { K(__VA_ARGS__); })
-inline hipError_t hipGetLastError() { return hipSuccess; }
+#define hipLaunchKernelGGL(K, G, B, SHM, STREAM, ...) ::lps_emu::launch(dim3(G), dim3(B), __PRETTY_FUNCTION__, [=]() { K(__VA_ARGS__); })
+inline hipError_t hipGetLastError() {
+  const hipError_t e = lps_emu::g_error;
+  lps_emu::g_error = hipSuccess;
+  return e;
+}
 inline hipError_t hipGetDevice(int* d) { *d = 0; return hipSuccess; }
 inline hipError_t hipDeviceGetAttribute(int* v, int, int) { *v = 256; return hipSuccess; }
 template <typename T>

@@ -333,3 +333,13 @@ def test_gradient_into_rows_of_a_wider_buffer(dev, n, dtype):
     assert bool((buf[:5, 3:3 + hidden] == times[:, None]).all())
     assert int(torch.count_nonzero(buf[5:, 3:3 + hidden])) == 0
     assert bool((buf[:, :3] == 7).all()) and bool((buf[:, 3 + hidden:] == 7).all())
+
+
+@pytest.mark.parametrize("vocab,hidden,dtype", [(4096 * 1024 + 1, 1, torch.bfloat16), (5000001, 3, torch.float32),
+                                                (4096 * 1024, 7, torch.float16), (1, 1, torch.float32)])
+def test_gradient_of_no_positions(dev, vocab, hidden, dtype):
+    """A new gradient of an empty batch is zeros, whatever the vocabulary and the memory held."""
+    torch.full((vocab, hidden), 3.0, dtype=dtype, device=dev)       # freed at once: the same memory
+    none = torch.empty((0,), dtype=torch.int64, device=dev)
+    got = lps.embedding_grad(none, torch.empty((0, hidden), dtype=dtype, device=dev), vocab)
+    assert got.shape == (vocab, hidden) and int(torch.count_nonzero(got)) == 0

@@ -1,0 +1,45 @@
+"""The vocabulary table's launches (CPU, no GPU): the C ABI compiled for x86 over
+the HIP emulation lists what it would launch, at sizes that no CPU run has memory
+for."""
+
+import struct
+from collections import namedtuple
+
+import pytest
+
+from tests.test_hostemu import _exec
+from tests.test_hostemu_table import run_table  # noqa: F401
+
+QUANTISE, LOOKUP, GRADIENT, HEAD, DEQUANTISE = 1, 2, 3, 4, 5
+F32, BF16, F16, MX4 = 0, 1, 2, 3
+ELAUNCH = 3
+
+Launch = namedtuple("Launch", "taken grid threads kernel")
+
+
+@pytest.fixture
+def launches(run_table, tmp_path, monkeypatch):  # noqa: F811
+    """The return code and launches of an entry point at given sizes."""
+    def call(entry, dtype, out_dtype, n, vocab, hidden, accumulate=0, cus=256):
+        inp, out, listed = tmp_path / "in.bin", tmp_path / "out.bin", tmp_path / "launches"
+        listed.write_text("")
+        inp.write_bytes(struct.pack("<16i", 5, entry, dtype, out_dtype, n, vocab, hidden, accumulate, *[0] * 8))
+        monkeypatch.setenv("LPS_EMU_LAUNCHES", str(listed))
+        monkeypatch.setenv("LPS_EMU_CUS", str(cus))
+        (rc,) = struct.unpack("<i", _exec(run_table, inp, out))
+        parts = [x.split(" ", 5) for x in listed.read_text().splitlines()]
+        return rc, [Launch(t == "1", (int(x), int(y), int(z)), int(b), f) for t, x, y, z, b, f in parts]
+    return call
+
+
+def fits(rc, made):
+    return rc == 0 and len(made) > 0 and all(m.taken for m in made)
+
+
+@pytest.mark.parametrize("vocab,hidden", [(4096 * 1024 + 1, 1), (1 << 23, 24), ((1 << 31) - 1, 1), (4096 * 1024, 1), (7, 40)])
+@pytest.mark.parametrize("out_dtype", [F32, BF16, F16])
+def test_empty_batch_into_a_new_gradient(launches, vocab, hidden, out_dtype):
+    """No position: the zeros alone, whatever the vocabulary; nothing when accumulating."""
+    rc, made = launches(GRADIENT, BF16, out_dtype, 0, vocab, hidden)
+    assert fits(rc, made) and len(made) == 1
+    assert launches(GRADIENT, BF16, out_dtype, 0, vocab, hidden, 1) == (0, [])
