@@ -119,8 +119,9 @@ hipError_t launch_grad(EmbGradParams P, hipStream_t s) {
     P.zero = !P.accumulate && bytes <= MX4_STREAM && P.n > 0;
     if (bytes > 0 && !P.zero) {
       hipLaunchKernelGGL((grad_zero_kernel<ODT>), dim3(fill_wgs(P, 256)), dim3(256), 0, s, P);
+      const hipError_t e = hipGetLastError();
+      if (e != hipSuccess || P.n == 0) return e;
     }
-    if (P.n == 0) return hipGetLastError();
     // about eight positions and 64 thousand values of zeros a workgroup, up to one on
     // each CU; more where it would own more ids than it can count
     const int64_t values = P.zero ? (int64_t)P.vocab * (P.hidden < 256 ? P.hidden : 256) : 0;
@@ -131,8 +132,13 @@ hipError_t launch_grad(EmbGradParams P, hipStream_t s) {
     hipLaunchKernelGGL((grad_small_kernel<GDT, ODT>), dim3(1u << lg, (unsigned)((P.hidden + 255) / 256)), dim3(256), 0, s, P);
     return hipGetLastError();
   }
+  // (each reads what the one before wrote: none follows a failed one)
   hipLaunchKernelGGL((grad_sort_kernel<ODT>), dim3((1u << P.lg_groups) + (P.accumulate ? 0 : fill_wgs(P, EG_NT))), dim3(EG_NT), 0, s, P);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
   hipLaunchKernelGGL((grad_tiles_kernel<GDT, ODT>), dim3((unsigned)((int64_t)P.tiles * P.slices)), dim3(256), 0, s, P);
+  e = hipGetLastError();
+  if (e != hipSuccess) return e;
   if (P.tiles > 1)
     hipLaunchKernelGGL((grad_join_kernel<ODT>), dim3((unsigned)((P.tiles - 1 + EG_JOIN - 1) / EG_JOIN), (unsigned)((P.hidden + 255) / 256)), dim3(256), 0, s, P);
   return hipGetLastError();

@@ -43,3 +43,12 @@ def test_empty_batch_into_a_new_gradient(launches, vocab, hidden, out_dtype):
     rc, made = launches(GRADIENT, BF16, out_dtype, 0, vocab, hidden)
     assert fits(rc, made) and len(made) == 1
     assert launches(GRADIENT, BF16, out_dtype, 0, vocab, hidden, 1) == (0, [])
+
+
+@pytest.mark.parametrize("n,vocab,hidden,failing", [(3000, 1000, 64, 0), (3000, 1000, 64, 1), (3000, 1000, 64, 2),
+                                                    (5, 100000, 1024, 0), (5, 1000, 64, 0)])
+def test_nothing_follows_a_failed_launch(launches, monkeypatch, n, vocab, hidden, failing):
+    """What a kernel would read is then not there: ids and counts of whatever the memory held."""
+    monkeypatch.setenv("LPS_EMU_FAIL", str(failing))
+    rc, made = launches(GRADIENT, BF16, F32, n, vocab, hidden)
+    assert rc == ELAUNCH and [m.taken for m in made] == [True] * failing + [False]
