@@ -30,7 +30,7 @@ constexpr int EG_OWN = 1024;        // ids a workgroup of the sort can own
 constexpr int EG_LIST = 3968;       // positions it keeps in LDS: as many as leave room for two workgroups a CU
 constexpr int EG_POS_BITS = 22;     // .. whose ids take the other 10
 constexpr int EG_SMAX = 1024;       // positions of a tile, at most
-constexpr int EG_FILL = 1 << 21;    // workgroups that write zeros: at most
+constexpr int EG_FILL = (1 << 21) - 8;   // workgroups that write zeros: at most
 constexpr int EG_JOIN = 8;          // tiles a joining workgroup looks at
 constexpr int EG_SMALL = 768;       // positions of the form without a sort
 

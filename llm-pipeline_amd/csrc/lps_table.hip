@@ -12,6 +12,7 @@ using namespace lps;
 namespace {
 
 constexpr int kMaxPositions = 1 << 30;   // of a gradient: its kernels count a little past them in 32 bits
+constexpr int64_t kMaxGroups = 0xFFFFFFFFu / 256;   // workgroups of 256: a launch has fewer than 2^32 threads
 
 bool aligned_to(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 size_t elem_bytes(int dtype) { return dtype == LPS_DTYPE_F32 ? 4 : 2; }
@@ -33,11 +34,25 @@ hipError_t launch_gather(GatherParams P, hipStream_t s) {
   // few rows: a long row over several workgroups
   const int chunks = (pieces + (1 << P.lg_tpr) - 1) >> P.lg_tpr;
   const unsigned y = wgs < 1024 ? (unsigned)(chunks < 65535 ? chunks : 65535) : 1u;
-  if (P.n * P.hidden * ElemBytes<ODT>::value > MX4_STREAM)
-    hipLaunchKernelGGL((gather_kernel<TDT, ODT, true>), dim3((unsigned)wgs, y), dim3(256), 0, s, P);
-  else
-    hipLaunchKernelGGL((gather_kernel<TDT, ODT, false>), dim3((unsigned)wgs, y), dim3(256), 0, s, P);
-  return hipGetLastError();
+  const bool past = P.n * P.hidden * ElemBytes<ODT>::value > MX4_STREAM;
+  // (rows that outgrow a launch: the next ones in another)
+  const int64_t most = kMaxGroups << (8 - P.lg_tpr);
+  for (int64_t left = P.n; left > 0; left -= most) {
+    P.n = left < most ? left : most;
+    const dim3 grid((unsigned)((P.n + (256 >> P.lg_tpr) - 1) >> (8 - P.lg_tpr)), y);
+    if (past) hipLaunchKernelGGL((gather_kernel<TDT, ODT, true>), grid, dim3(256), 0, s, P);
+    else hipLaunchKernelGGL((gather_kernel<TDT, ODT, false>), grid, dim3(256), 0, s, P);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    P.out = static_cast<char*>(P.out) + P.n * P.out_stride * ElemBytes<ODT>::value;
+    if (P.ids) {
+      P.ids = static_cast<const char*>(P.ids) + P.n * P.id_bytes;
+    } else {
+      P.table = static_cast<const char*>(P.table) + P.n * P.table_stride * (TDT == DT_MX4 ? 1 : ElemBytes<TDT>::value);
+      if (P.scales) P.scales += P.n * P.scales_stride;
+    }
+  }
+  return hipSuccess;
 }
 template <int TDT>
 hipError_t dispatch_gather(int out_dtype, const GatherParams& P, hipStream_t s) {
@@ -51,10 +66,21 @@ hipError_t dispatch_gather(int out_dtype, const GatherParams& P, hipStream_t s) 
 template <int DT>
 hipError_t launch_quantize(Mx4Params P, hipStream_t s) {
   P.lg_tpr = lg_threads_per_row(4 * P.blocks);
-  const dim3 grid((unsigned)(((int64_t)P.rows + (256 >> P.lg_tpr) - 1) >> (8 - P.lg_tpr)));
-  if ((int64_t)P.rows * P.blocks * 16 > MX4_STREAM) hipLaunchKernelGGL((mx4_quantize_kernel<DT, true>), grid, dim3(256), 0, s, P);
-  else hipLaunchKernelGGL((mx4_quantize_kernel<DT, false>), grid, dim3(256), 0, s, P);
-  return hipGetLastError();
+  const bool past = (int64_t)P.rows * P.blocks * 16 > MX4_STREAM;
+  // (rows that outgrow a launch: the next ones in another)
+  const int64_t most = kMaxGroups << (8 - P.lg_tpr);
+  for (int64_t left = P.rows; left > 0; left -= most) {
+    P.rows = (int)(left < most ? left : most);
+    const dim3 grid((unsigned)(((int64_t)P.rows + (256 >> P.lg_tpr) - 1) >> (8 - P.lg_tpr)));
+    if (past) hipLaunchKernelGGL((mx4_quantize_kernel<DT, true>), grid, dim3(256), 0, s, P);
+    else hipLaunchKernelGGL((mx4_quantize_kernel<DT, false>), grid, dim3(256), 0, s, P);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    P.x = static_cast<const char*>(P.x) + P.rows * P.x_stride * ElemBytes<DT>::value;
+    P.codes += P.rows * P.codes_stride;
+    P.scales += P.rows * P.scales_stride;
+  }
+  return hipSuccess;
 }
 
 int check_mx4(const lps_mx4_args* a) {
@@ -105,7 +131,8 @@ EgWs eg_workspace(int n, int vocab, int hidden) {
 }
 
 // Workgroups of `threads` that zero all rows: 16 bytes a thread, whole eights, up to
-// EG_FILL (a launch has fewer than 2^32 threads).
+// EG_FILL (a launch has fewer than 2^32 threads, the sort's at most 2^21 workgroups
+// of 1024 among them).
 unsigned fill_wgs(const EmbGradParams& P, int threads) {
   const int64_t eights = (P.fill_rows * P.fill_lines + 8 * threads - 1) / (8 * threads);
   return eights < EG_FILL / 8 ? 8 * (unsigned)eights : (unsigned)EG_FILL;
@@ -279,7 +306,7 @@ int lps_embedding_grad(const lps_embedding_grad_args* a, void* stream) {
   P.fill_bytes = whole ? a->vocab * row_bytes : row_bytes;
   P.fill_lines = aligned_to(a->out, 16) && P.out_stride * elem_bytes(a->out_dtype) % 16 == 0 ? (P.fill_bytes + 15) / 16
                                                                                             : (P.fill_bytes + 14) / 16 + 1;
-  if ((int64_t)P.tiles * P.slices > 0x7FFFFFFF || (a->hidden + 255) / 256 > 65535) return LPS_EINVAL;
+  if ((int64_t)P.tiles * P.slices > kMaxGroups || (a->hidden + 255) / 256 > 65535) return LPS_EINVAL;
   P.count = reinterpret_cast<int*>(ws + w.count);
   P.sid = reinterpret_cast<int*>(ws + w.sid);
   P.spos = reinterpret_cast<int*>(ws + w.spos);

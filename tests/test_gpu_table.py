@@ -343,3 +343,33 @@ def test_gradient_of_no_positions(dev, vocab, hidden, dtype):
     none = torch.empty((0,), dtype=torch.int64, device=dev)
     got = lps.embedding_grad(none, torch.empty((0, hidden), dtype=dtype, device=dev), vocab)
     assert got.shape == (vocab, hidden) and int(torch.count_nonzero(got)) == 0
+
+
+def test_rows_past_a_grid(dev):
+    """More rows than the threads of one launch can take, 16 to a row: every one is
+    there (values that their block's scale leaves exact)."""
+    rows = (1 << 28) + 5
+    x = torch.tensor([1.0, 1.5, -2.0, 3.0, -0.75, 0.0, 48.0], dtype=torch.bfloat16, device=dev)
+    ids = torch.arange(rows, dtype=torch.int32, device=dev).remainder_(7)
+    all_rows = torch.empty((rows, 1), dtype=torch.bfloat16, device=dev)
+    for i in range(0, rows, 1 << 24):
+        all_rows[i:i + (1 << 24), 0] = x[ids[i:i + (1 << 24)].long()]
+    assert torch.equal(lps.embedding(ids, x[:, None]), all_rows)
+    t = lps.mx4_quantize(all_rows)
+    assert torch.equal(lps.mx4_dequantize(t), all_rows)
+
+
+def test_gradient_of_a_huge_vocabulary(dev):
+    """The sort's and the zeros' workgroups together at their most: 34 GB of zeros but
+    for the ids' rows."""
+    vocab, hidden, n = (1 << 30) + 1, 8, 900
+    g = torch.Generator().manual_seed(21)
+    ids = torch.randint(0, vocab, (n,), generator=g)
+    ids[:3] = torch.tensor([0, vocab - 1, vocab - 1])
+    torch.full((vocab, hidden), 3.0, device=dev)                    # freed at once: the same memory
+    got = lps.embedding_grad(ids.to(dev), torch.ones((n, hidden), device=dev), vocab)
+    rows, times = ids.unique(return_counts=True)
+    assert bool((got[rows.to(dev)].cpu() == times[:, None]).all())
+    got[rows.to(dev)] = 0
+    for i in range(0, vocab, 1 << 27):
+        assert int(torch.count_nonzero(got[i:i + (1 << 27)])) == 0

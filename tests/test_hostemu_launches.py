@@ -52,3 +52,36 @@ def test_nothing_follows_a_failed_launch(launches, monkeypatch, n, vocab, hidden
     monkeypatch.setenv("LPS_EMU_FAIL", str(failing))
     rc, made = launches(GRADIENT, BF16, F32, n, vocab, hidden)
     assert rc == ELAUNCH and [m.taken for m in made] == [True] * failing + [False]
+
+
+MANY = 1 << 28    # rows of 16 threads each: 2^32 threads
+
+
+@pytest.mark.parametrize("rows,hidden,parts", [(MANY - 16, 1, 1), (MANY - 15, 1, 2), (MANY + 5, 1, 2), ((1 << 31) - 1, 1, 9),
+                                               ((1 << 24) - 1, 2049, 1), (1 << 24, 2049, 2), (1 << 24, 4096, 2)])
+@pytest.mark.parametrize("entry,dtype,out_dtype", [(QUANTISE, BF16, 0), (DEQUANTISE, F16, 0), (LOOKUP, BF16, BF16),
+                                                   (LOOKUP, MX4, F16)])
+def test_rows_past_a_grid(launches, entry, dtype, out_dtype, rows, hidden, parts):
+    """More rows than fewer than 2^32 threads can take: by several launches that cover them."""
+    rc, made = launches(entry, dtype, out_dtype, rows, rows, hidden)
+    assert fits(rc, made) and len(made) == parts
+    assert sum(m.grid[0] * m.threads for m in made) >= rows * (16 if hidden == 1 else 256)
+
+
+def test_fp32_rows_past_a_grid(launches):
+    """A thread stores half as many fp32 values: 256 threads a row from 1025 columns."""
+    rc, made = launches(DEQUANTISE, F32, 0, 1 << 24, 1, 1025)
+    assert fits(rc, made) and len(made) == 2
+
+
+@pytest.mark.parametrize("vocab,hidden,dtype", [((1 << 30) + 1, 8, F32), ((1 << 31) - 1, 4, F32), ((1 << 31) - 1, 64, BF16)])
+@pytest.mark.parametrize("n", [1, 900, 20000])
+def test_gradients_of_huge_vocabularies(launches, n, vocab, hidden, dtype):
+    """The sort's workgroups (one to 1024 ids) and those of the zeros beside them in one grid."""
+    rc, made = launches(GRADIENT, BF16, dtype, n, vocab, hidden)
+    assert fits(rc, made) and made[0].grid[0] > 1 << 21
+
+
+def test_gradients_of_more_tiles_than_a_grid(launches):
+    """Sizes past it are refused before any launch."""
+    assert launches(GRADIENT, BF16, F32, 1 << 30, 1000, 16 * 2048 + 1) == (1, [])
