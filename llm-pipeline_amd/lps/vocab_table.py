@@ -13,6 +13,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _device as D
 from . import _lib
@@ -90,6 +91,11 @@ def _flat_rows(x: torch.Tensor) -> torch.Tensor:
 def _same_device(a: torch.Tensor, b: torch.Tensor, what: str) -> None:
     if a.get_device() != b.get_device():
         raise ValueError(f"{what} are on different devices: {a.device}, {b.device}")
+
+
+def _has_tangent(t: torch.Tensor) -> bool:
+    """Whether t carries a forward-mode derivative (it can where a level of them is open)."""
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
 
 
 def _call(name: str, args: bytes, device: torch.device) -> None:
@@ -203,13 +209,19 @@ def _embedding(ids: torch.Tensor, table: Union[torch.Tensor, Mx4Tensor], scale: 
 
 
 class _Embedding(torch.autograd.Function):
-    """The lookup with its gradient in the table."""
+    """The lookup with its derivatives in the table: it is linear in it."""
 
     @staticmethod
     def forward(ctx, ids, table, scale, out_dtype):
         ctx.save_for_backward(ids)
-        ctx.vocab, ctx.scale, ctx.dtype = table.shape[0], scale, table.dtype
+        ctx.save_for_forward(ids)
+        ctx.vocab, ctx.scale, ctx.dtype, ctx.out_dtype = table.shape[0], scale, table.dtype, out_dtype
         return _embedding(ids, table, scale, out_dtype)
+
+    @staticmethod
+    def jvp(ctx, _, tangent, *__):
+        (ids,) = ctx.saved_tensors
+        return embedding(ids, tangent, ctx.scale, ctx.out_dtype)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -224,8 +236,9 @@ def embedding(ids: torch.Tensor, table: Union[torch.Tensor, Mx4Tensor], scale: f
     a table ``[V, H]`` in float32, bfloat16, float16 or 4 bits; fp32 arithmetic,
     rounded once to ``out_dtype`` (default: the table's type, bfloat16 for 4
     bits).  Ids outside ``[0, V)``, -1 among them, give zeros.  A table that
-    requires a gradient gets it from ``embedding_grad``."""
-    if isinstance(table, torch.Tensor) and table.requires_grad and torch.is_grad_enabled():
+    requires a gradient gets it from ``embedding_grad``; the forward-mode
+    derivative of one that carries a tangent is the tangent's lookup."""
+    if isinstance(table, torch.Tensor) and ((table.requires_grad and torch.is_grad_enabled()) or _has_tangent(table)):
         return _Embedding.apply(ids, table, scale, out_dtype)
     return _embedding(ids, table, scale, out_dtype)
 

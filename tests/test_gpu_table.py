@@ -373,3 +373,17 @@ def test_gradient_of_a_huge_vocabulary(dev):
     got[rows.to(dev)] = 0
     for i in range(0, vocab, 1 << 27):
         assert int(torch.count_nonzero(got[i:i + (1 << 27)])) == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_lookup_tangent(dev, dtype):
+    """Forward mode: the tangent's lookup, of a table that requires a gradient and of one that does not."""
+    from torch.autograd import forward_ad
+    g = torch.Generator().manual_seed(14)
+    ids = torch.randint(-1, 13, (3, 7), generator=g).to(dev)
+    w, t = torch.randn((12, 40), generator=g).to(dev, dtype), torch.randn((12, 40), generator=g).to(dev, dtype)
+    with forward_ad.dual_level():
+        for table in (w, w.clone().requires_grad_()):
+            out = forward_ad.unpack_dual(lps.embedding(ids, forward_ad.make_dual(table, t), scale=1.5))
+            assert torch.equal(out.primal, lps.embedding(ids, w, scale=1.5))
+            assert torch.equal(out.tangent, lps.embedding(ids, t, scale=1.5))
