@@ -17,7 +17,7 @@ import torch
 
 from . import _device as D
 from . import _lib
-from .vocab_table import Mx4Tensor, _call, _on_gpu, _same_device, _sizes
+from .vocab_table import Mx4Tensor, _call, _no_derivative, _on_gpu, _same_device, _sizes
 
 _pack_mx4 = _lib.packer(_lib.LmHeadMx4Args)
 
@@ -28,11 +28,13 @@ def lm_head(hidden: Union[torch.Tensor, Mx4Tensor], weight: Union[torch.Tensor, 
     accumulation, stored in ``out_dtype``, default the input dtype).  Inputs:
     bf16 or fp16, the same dtype, ``H`` a multiple of 16.  ``return_stats``
     also returns ``[..., ceil(V / 128), 2]`` float32 block statistics
-    ``(max, sum(exp(v - max)))`` of the stored logits.
+    ``(max, sum(exp(v - max)))`` of the stored logits.  The logits carry no
+    gradient.
 
     ``weight`` may be 4-bit (``mx4_quantize``): then ``H`` is any number,
     ``hidden`` bf16, fp16 or 4-bit itself, and ``out_dtype`` bfloat16 by default
-    for 4-bit ``hidden``.  The products are exact and summed in fp32."""
+    for 4-bit ``hidden``.  The products are exact and summed in fp32.  A 16-bit
+    ``hidden`` that asks for a derivative is refused."""
     if isinstance(weight, Mx4Tensor) or isinstance(hidden, Mx4Tensor):
         return _lm_head_mx4(hidden, weight, out_dtype, return_stats)
     D.require_device(hidden, "hidden")
@@ -102,6 +104,7 @@ def _lm_head_mx4(hidden, weight, out_dtype, return_stats):
         _on_gpu(hidden, "hidden")
         if hidden.dtype is not torch.bfloat16 and hidden.dtype is not torch.float16:
             raise TypeError("hidden must be bfloat16, float16 or an Mx4Tensor")
+        _no_derivative(hidden, "hidden", "lm_head over a 4-bit weight")
         code, od = D.code_of(hidden.dtype), out_dtype or hidden.dtype
         lead, width = hidden.shape[:-1], hidden.shape[-1] if hidden.dim() else 0
         x, xp, xss = hidden, 0, 0

@@ -98,6 +98,13 @@ def _has_tangent(t: torch.Tensor) -> bool:
     return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
 
 
+def _no_derivative(t: torch.Tensor, name: str, call: str) -> None:
+    """Raises where t asks for a derivative: the call has none, and would lose it."""
+    if (t.requires_grad and torch.is_grad_enabled()) or _has_tangent(t):
+        raise ValueError(f"{call} has no derivative in {name}, which requires a gradient or carries a tangent; "
+                         "detach it, or call without gradients")
+
+
 def _call(name: str, args: bytes, device: torch.device) -> None:
     """The entry point on the device's current stream; raises for its return code."""
     fn = getattr(_lib.load(), name)
@@ -124,7 +131,8 @@ def mx4_quantize(x: torch.Tensor) -> Mx4Tensor:
     magnitude)) - 2, -126), and the codes of the nearest of 0, 0.5, 1, 1.5, 2, 3,
     4, 6 to ``|x| / 2^s`` (ties to the even code, 6 above it; signs are kept).  A
     block with a value that is not finite becomes NaN.  ``H`` need not be a
-    multiple of 32."""
+    multiple of 32.  Codes and scales are whole numbers: they carry no gradient of
+    ``x``."""
     _on_gpu(x, "x")
     code = D.code_of(x.dtype)
     if x.dim() < 1 or x.shape[-1] < 1:
@@ -252,10 +260,12 @@ def embedding_grad(ids: torch.Tensor, grad: torch.Tensor, vocab: int, scale: flo
     A new tensor ``[vocab, H]`` of ``dtype`` (default: ``grad``'s), or, with
     ``out``, added to ``out [vocab, H]`` (of which the rows without a position are
     left alone) and ``out`` returned.  The order of the sum depends on ids and
-    sizes alone: equal calls give equal bits."""
+    sizes alone: equal calls give equal bits.  It has no derivative itself: a
+    ``grad`` or ``out`` that asks for one is refused."""
     flat = _ids(ids)
     _on_gpu(grad, "grad")
     code = D.code_of(grad.dtype)
+    _no_derivative(grad, "grad", "embedding_grad")
     if grad.dim() != ids.dim() + 1 or grad.shape[:-1] != ids.shape or grad.shape[-1] < 1:
         raise ValueError(f"ids [...] and grad [..., H] expected; got {tuple(ids.shape)}, {tuple(grad.shape)}")
     if vocab < 1:
@@ -277,8 +287,7 @@ def embedding_grad(ids: torch.Tensor, grad: torch.Tensor, vocab: int, scale: flo
         if out.shape != (vocab, hidden) or (hidden > 1 and out.stride(1) != 1) or (vocab > 1 and out.stride(0) < hidden):
             raise ValueError(f"out [{vocab}, {hidden}] with rows of neighbouring elements expected; got "
                              f"{tuple(out.shape)}, strides {out.stride()}")
-        if out.requires_grad and torch.is_grad_enabled():
-            raise ValueError("out requires a gradient; pass its .grad, or a detached tensor")
+        _no_derivative(out, "out", "embedding_grad")
         res = out
     need = _lib.load().lps_embedding_grad_workspace_bytes(n, vocab, hidden)
     ws = torch.empty((need,), dtype=torch.uint8, device=device) if need else None

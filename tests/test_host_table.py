@@ -36,3 +36,57 @@ def test_tangent_of_a_lookup(plain_lookup, dtype, out_dtype, grad_mode):
         assert forward_ad.unpack_dual(lps.embedding(IDS, w)).tangent is None
         both = lps.embedding(IDS, forward_ad.make_dual(w.clone().requires_grad_(), t))
         assert both.requires_grad == grad_mode and forward_ad.unpack_dual(both).tangent is not None
+
+
+@pytest.fixture
+def anywhere(monkeypatch):
+    """CPU tensors pass for the GPU's; the entry points' calls are kept, not made."""
+    from lps import lmhead
+    calls = []
+    for m in (T, lmhead):
+        monkeypatch.setattr(m, "_on_gpu", lambda t, name: None)
+        monkeypatch.setattr(m, "_call", lambda name, args, device: calls.append((name, args)))
+    return calls
+
+
+def _weight(V, H):
+    n = -(-H // 32)
+    return lps.Mx4Tensor(torch.zeros((V, 16 * n), dtype=torch.uint8), torch.full((V, n), 127, dtype=torch.uint8), H)
+
+
+def test_derivatives_that_a_call_does_not_have(anywhere):
+    """An input that asks for one is refused, not answered without it; the same call
+    without gradients, or of a detached input, is made."""
+    w = _weight(8, 64)
+    x, grad, out = torch.zeros((2, 64), dtype=torch.bfloat16), torch.zeros((2, 64)), torch.zeros((8, 64))
+    ids = torch.tensor([1, 3])
+    cases = [(x, lambda t: lps.lm_head(t, w)), (x, lambda t: lps.lm_head(t, w, return_stats=True)),
+             (grad, lambda t: lps.embedding_grad(ids, t, 8)), (out, lambda t: lps.embedding_grad(ids, grad, 8, out=t))]
+    for t, call in cases:
+        needs = t.clone().requires_grad_()
+        with pytest.raises(ValueError, match="derivative|gradient"):
+            call(needs)
+        with forward_ad.dual_level(), pytest.raises(ValueError, match="derivative"):
+            call(forward_ad.make_dual(t, torch.ones_like(t)))
+        assert not anywhere
+        with torch.no_grad():
+            call(needs)
+        call(needs.detach())
+        with forward_ad.dual_level():
+            call(t)
+        assert len(anywhere) == 3
+        anywhere.clear()
+
+
+def test_tangent_of_a_lookups_gradient(plain_lookup, anywhere):
+    """Forward over reverse is refused too."""
+    w = torch.ones((5, 8)).requires_grad_()
+    with forward_ad.dual_level(), pytest.raises(ValueError, match="derivative"):
+        out = lps.embedding(IDS, forward_ad.make_dual(w, torch.ones((5, 8))))
+        (out * out).sum().backward()
+
+
+def test_quantised_values_have_no_gradient(anywhere):
+    """Codes and scales are whole numbers: a weight that requires a gradient is quantised without one."""
+    t = lps.mx4_quantize(torch.nn.Parameter(torch.ones((4, 40))))
+    assert not t.codes.requires_grad and not t.scales.requires_grad and len(anywhere) == 1
