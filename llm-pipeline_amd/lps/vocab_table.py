@@ -295,4 +295,6 @@ def embedding_grad(ids: torch.Tensor, grad: torch.Tensor, vocab: int, scale: flo
           _pack_grad(flat.data_ptr(), g.data_ptr(), res.data_ptr(), flat.element_size(), code, out_code, n, vocab, hidden,
                      g.stride(0) if n > 1 else hidden, res.stride(0) if vocab > 1 else hidden, scale,
                      0 if out is None else 1, D.ptr(ws), need), device)
+    if out is not None:
+        torch.autograd.graph.increment_version(out)   # written behind autograd's back
     return res

@@ -90,3 +90,19 @@ def test_quantised_values_have_no_gradient(anywhere):
     """Codes and scales are whole numbers: a weight that requires a gradient is quantised without one."""
     t = lps.mx4_quantize(torch.nn.Parameter(torch.ones((4, 40))))
     assert not t.codes.requires_grad and not t.scales.requires_grad and len(anywhere) == 1
+
+
+def test_out_counts_as_written(anywhere):
+    """A graph that saved out must not use the changed values."""
+    ids, grad, out = torch.tensor([1, 3]), torch.zeros((2, 8)), torch.ones((4, 8))
+    w = torch.ones((4, 8)).requires_grad_()
+    loss = (w * out).sum()                            # saves out
+    lps.embedding_grad(ids, grad, 4, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    view = torch.ones((4, 20))
+    before = view._version
+    lps.embedding_grad(ids, grad, 4, out=view[:, 3:11])
+    assert view._version > before
+    with torch.inference_mode():
+        lps.embedding_grad(ids, grad, 4, out=torch.ones((4, 8)))
