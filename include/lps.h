@@ -441,7 +441,7 @@ int lps_embedding(const lps_embedding_args* args, void* stream);
  * (ids outside [0, vocab) add nothing), on top of out[v] with accumulate (rows
  * without an id are then not touched).  Summed in fp32, rounded once, in an
  * order that depends on ids and sizes alone: equal calls give equal bits.  At most
- * 2^30 positions.
+ * 2^30 positions.  out shares no memory with ids and grad.
  * workspace: lps_embedding_grad_workspace_bytes(n, vocab, hidden) bytes (0 for few
  * positions), 16-byte aligned, of any content; calls that overlap in time must not
  * share it. */

@@ -105,6 +105,20 @@ def _no_derivative(t: torch.Tensor, name: str, call: str) -> None:
                          "detach it, or call without gradients")
 
 
+def _share_memory(a, b) -> bool:
+    """Whether two sets of rows, each (address, rows, bytes from row to row, bytes of
+    one), have a byte in common.  Rows of one set do not overlap each other."""
+    if a[1] > b[1]:
+        a, b = b, a
+    (p, n, s, k), (q, m, t, j) = a, b
+    if n == 0 or p + (n - 1) * s + k <= q or q + (m - 1) * t + j <= p:
+        return False
+    # of each row of the smaller set: the last row of the other that begins before its end
+    x = p - q + s * torch.arange(n, dtype=torch.int64, device="cpu")
+    last = torch.div(x + (k - 1), max(t, 1), rounding_mode="floor").clamp_(max=m - 1)
+    return bool(((last >= 0) & (last * t + j > x)).any())
+
+
 def _call(name: str, args: bytes, device: torch.device) -> None:
     """The entry point on the device's current stream; raises for its return code."""
     fn = getattr(_lib.load(), name)
@@ -259,7 +273,8 @@ def embedding_grad(ids: torch.Tensor, grad: torch.Tensor, vocab: int, scale: flo
 
     A new tensor ``[vocab, H]`` of ``dtype`` (default: ``grad``'s), or, with
     ``out``, added to ``out [vocab, H]`` (of which the rows without a position are
-    left alone) and ``out`` returned.  The order of the sum depends on ids and
+    left alone) and ``out`` returned (it shares no memory with ``grad`` and
+    ``ids``).  The order of the sum depends on ids and
     sizes alone: equal calls give equal bits.  It has no derivative itself: a
     ``grad`` or ``out`` that asks for one is refused."""
     flat = _ids(ids)
@@ -289,12 +304,17 @@ def embedding_grad(ids: torch.Tensor, grad: torch.Tensor, vocab: int, scale: flo
                              f"{tuple(out.shape)}, strides {out.stride()}")
         _no_derivative(out, "out", "embedding_grad")
         res = out
+    gs, rs = g.stride(0) if n > 1 else hidden, res.stride(0) if vocab > 1 else hidden
+    if out is not None:
+        rows = (res.data_ptr(), vocab, rs * res.element_size(), hidden * res.element_size())
+        if (_share_memory((g.data_ptr(), n, gs * g.element_size(), hidden * g.element_size()), rows)
+                or _share_memory((flat.data_ptr(), 1 if n else 0, 0, n * flat.element_size()), rows)):
+            raise ValueError("out overlaps grad or ids in memory")
     need = _lib.load().lps_embedding_grad_workspace_bytes(n, vocab, hidden)
     ws = torch.empty((need,), dtype=torch.uint8, device=device) if need else None
     _call("lps_embedding_grad",
           _pack_grad(flat.data_ptr(), g.data_ptr(), res.data_ptr(), flat.element_size(), code, out_code, n, vocab, hidden,
-                     g.stride(0) if n > 1 else hidden, res.stride(0) if vocab > 1 else hidden, scale,
-                     0 if out is None else 1, D.ptr(ws), need), device)
+                     gs, rs, scale, 0 if out is None else 1, D.ptr(ws), need), device)
     if out is not None:
         torch.autograd.graph.increment_version(out)   # written behind autograd's back
     return res

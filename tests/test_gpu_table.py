@@ -387,3 +387,18 @@ def test_lookup_tangent(dev, dtype):
             out = forward_ad.unpack_dual(lps.embedding(ids, forward_ad.make_dual(table, t), scale=1.5))
             assert torch.equal(out.primal, lps.embedding(ids, w, scale=1.5))
             assert torch.equal(out.tangent, lps.embedding(ids, t, scale=1.5))
+
+
+def test_gradient_out_beside_its_inputs(dev):
+    """out and grad in one buffer: refused where they overlap, right where their rows alternate."""
+    g = torch.Generator().manual_seed(15)
+    ids = torch.randint(0, 30, (30,), generator=g)
+    both = torch.randn((30, 40), generator=g)
+    buf = both.to(dev)
+    with pytest.raises(ValueError, match="overlap"):
+        lps.embedding_grad(ids.to(dev), buf[:, 8:28], 30, out=buf[:, 20:])
+    before = buf._version
+    lps.embedding_grad(ids.to(dev), buf[:, :20], 30, out=buf[:, 20:])
+    want, bound = R.gradient(ids, both[:, :20], 30, 1.0, both[:, 20:], torch.float32)
+    assert buf._version > before and torch.equal(buf[:, :20].cpu(), both[:, :20])
+    assert bool(((buf[:, 20:].double().cpu() - want).abs() <= bound).all())

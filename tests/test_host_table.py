@@ -106,3 +106,45 @@ def test_out_counts_as_written(anywhere):
     assert view._version > before
     with torch.inference_mode():
         lps.embedding_grad(ids, grad, 4, out=torch.ones((4, 8)))
+
+
+def _bytes_of(t):
+    """Every byte address that t's elements take."""
+    at = [t.data_ptr()]
+    for n, s in zip(t.shape, t.stride()):
+        at = [a + i * s * t.element_size() for a in at for i in range(n)]
+    return {a + k for a in at for k in range(t.element_size())}
+
+
+def test_out_that_shares_memory_with_its_inputs(anywhere):
+    """Refused where a byte is shared, and only there: rows between each other's are two tensors."""
+    buf = torch.zeros(4096)
+    sizes = [(1, 8, 8), (4, 8, 8), (4, 8, 20), (5, 3, 20), (3, 8, 28), (6, 5, 9), (4, 12, 20)]
+    seen = set()
+    for V, H, s in sizes:
+        out = buf[200:].as_strided((V, H), (s, 1))
+        for n, h, t in sizes:
+            if h != H:
+                continue
+            for off in range(120, 360, 4):
+                grad = buf[off:].as_strided((n, H), (t, 1))
+                shared = bool(_bytes_of(out) & _bytes_of(grad))
+                between = not shared and off < 200 + V * s and off + n * t > 200
+                seen.add((shared, between))
+                call = lambda: lps.embedding_grad(torch.zeros(n, dtype=torch.int64), grad, V, out=out)  # noqa: E731
+                if shared:
+                    with pytest.raises(ValueError, match="overlap"):
+                        call()
+                else:
+                    call()
+    assert seen == {(True, False), (False, False), (False, True)}
+    half = buf.view(torch.bfloat16)
+    with pytest.raises(ValueError, match="overlap"):
+        lps.embedding_grad(torch.tensor([0, 1]), half[:16].view(2, 8), 4, out=buf[:32].view(4, 8))
+    ids = buf.view(torch.int64)[:4]
+    with pytest.raises(ValueError, match="overlap"):
+        lps.embedding_grad(ids, torch.zeros((4, 8)), 4, out=buf[6:38].view(4, 8))
+    lps.embedding_grad(ids, torch.zeros((4, 8)), 4, out=buf[8:40].view(4, 8))
+    # a gradient that is copied first (every position the same row) is read before out is written
+    lps.embedding_grad(torch.zeros(3, dtype=torch.int64), buf[:8].expand(3, 8), 4, out=buf[:32].view(4, 8))
+    lps.embedding_grad(torch.zeros(0, dtype=torch.int64), buf[:0].view(0, 8), 4, out=buf[:32].view(4, 8))
