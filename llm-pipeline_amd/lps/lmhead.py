@@ -117,9 +117,13 @@ def _lm_head_mx4(hidden, weight, out_dtype, return_stats):
     if code != _lib.LPS_DTYPE_MX4:
         r, e = x.stride()
         # rows on 16-byte lines: a copy that lies so
-        if (e != 1 and H > 1) or x.data_ptr() % 16 or (M > 1 and (r % 8 or not H <= r <= _MX4_MAX_STRIDE // 2)):
+        if (e != 1 and H > 1) or x.data_ptr() % 16 or (M > 1 and (r % 8 or not H <= r <= max(_MX4_MAX_STRIDE // 2, H + 7))):
             x = torch.empty((M, H + -H % 8), dtype=x.dtype, device=x.device)[:, :H].copy_(x)
+    elif M > 1 and x.stride(0) > _MX4_MAX_STRIDE:
+        x = x.contiguous()
     w, ws = weight.rows()
+    if w.shape[0] > 1 and w.stride(0) > _MX4_MAX_STRIDE:
+        w = w.contiguous()
     ws = _words(ws)
     device, V = w.device, w.shape[0]
     _sizes(M, V, H)
@@ -127,9 +131,15 @@ def _lm_head_mx4(hidden, weight, out_dtype, return_stats):
     out = torch.empty((M, V), dtype=od, device=device)
     G = (V + _lib.LMHEAD_BLOCK_COLS - 1) // _lib.LMHEAD_BLOCK_COLS
     stats = torch.empty((M, G, 2), dtype=torch.float32, device=device) if return_stats else None
-    if M:
+    # (16-bit rows of more than 8 MiB: one to a call)
+    step = M if code == _lib.LPS_DTYPE_MX4 or M < 2 or x.stride(0) <= _MX4_MAX_STRIDE // 2 else 1
+    for m in range(0, M, step or 1):
+        if m:
+            xm, op, sp = x[m:].data_ptr(), out[m:].data_ptr(), D.ptr(None if stats is None else stats[m:])
+        else:
+            xm, op, sp = x.data_ptr(), out.data_ptr(), D.ptr(stats)
         _call("lps_lm_head_mx4",
-              _pack_mx4(x.data_ptr(), xp, w.data_ptr(), ws.data_ptr(), out.data_ptr(), D.ptr(stats), code, out_code, M, V, H,
+              _pack_mx4(xm, xp, w.data_ptr(), ws.data_ptr(), op, sp, code, out_code, step, V, H,
                         x.stride(0), xss, w.stride(0), ws.stride(0), V), device)
     if len(lead) != 1:
         out = out.reshape(*lead, V)

@@ -200,3 +200,30 @@ def test_refusals(dev):
         lps.lm_head(x, lps.Mx4Tensor(t.codes.int(), t.scales, 64))
     with pytest.raises(RuntimeError, match="ROCm device"):
         lps.lm_head(x.cpu(), t)
+
+
+@pytest.mark.parametrize("M,H,xs,dtype", [
+    (3, (1 << 22) + 8, (1 << 22) + 8, torch.float16), (2, (1 << 22) + 3, (1 << 22) + 3, torch.bfloat16),
+    (1, 1 << 24, 1 << 24, torch.bfloat16), (2, 1 << 24, 1 << 23, "mx4"), (5, 96, (1 << 22) + 8, torch.bfloat16),
+    (5, 96, (1 << 23) + 16, "mx4")])
+def test_head_rows_far_apart(dev, M, H, xs, dtype):
+    """Long rows and rows more than 8 MiB apart: sums of whole numbers, the same bits as in 64."""
+    g = torch.Generator().manual_seed(M + H)
+    V, n = 3, -(-H // 32)
+    codes = torch.randint(0, 256, (V, 16 * n), generator=g).to(torch.uint8)
+    scales = torch.full((V, n), 128, dtype=torch.uint8)               # values of -12 .. 12
+    wide = torch.zeros((V, (1 << 23) + 16), dtype=torch.uint8, device=dev)
+    wide[:, :16 * n] = codes.to(dev)
+    at = torch.randint(0, H, (M, 500), generator=g)
+    at[:, 0], at[:, 1] = H - 1, 0
+    x = torch.zeros((M, H)).scatter_(1, at, torch.randint(1, 3, (M, 500), generator=g).float())
+    if dtype == "mx4":
+        c, s = R.quantise(x)
+        rows = torch.zeros(((M - 1) * xs + 16 * n,), dtype=torch.uint8, device=dev).as_strided((M, 16 * n), (xs, 1))
+        arg = lps.Mx4Tensor(rows.copy_(c), s.to(dev), H)
+    else:
+        arg = torch.zeros(((M - 1) * xs + H,), dtype=dtype, device=dev).as_strided((M, H), (xs, 1)).copy_(x)
+    out, stats = lps.lm_head(arg, lps.Mx4Tensor(wide[:, :16 * n], scales.to(dev), H), out_dtype=torch.float32, return_stats=True)
+    ref = torch.stack([x.double() @ R.values(codes[v:v + 1], scales[v:v + 1], H)[0] for v in range(V)], 1)
+    assert torch.equal(out.double().cpu(), ref)
+    assert torch.equal(stats[..., 0].double().cpu(), ref.amax(1, keepdim=True))

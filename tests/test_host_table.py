@@ -148,3 +148,36 @@ def test_out_that_shares_memory_with_its_inputs(anywhere):
     # a gradient that is copied first (every position the same row) is read before out is written
     lps.embedding_grad(torch.zeros(3, dtype=torch.int64), buf[:8].expand(3, 8), 4, out=buf[:32].view(4, 8))
     lps.embedding_grad(torch.zeros(0, dtype=torch.int64), buf[:0].view(0, 8), 4, out=buf[:32].view(4, 8))
+
+
+def _strided(V, n, s):
+    """uint8 [V, n], rows s bytes apart."""
+    return torch.zeros((V - 1) * s + n, dtype=torch.uint8).as_strided((V, n), (s, 1))
+
+
+@pytest.mark.parametrize("M,H,xs,dtype", [
+    (3, 1 << 22, 1 << 22, torch.bfloat16), (3, (1 << 22) + 8, (1 << 22) + 8, torch.float16),
+    (2, (1 << 22) + 3, (1 << 22) + 3, torch.bfloat16), (2, 64, (1 << 22) + 8, torch.bfloat16),
+    (2, 64, (1 << 23) + 16, "mx4"), (3, 64, 32, "mx4"), (1, (1 << 24), 1 << 24, torch.bfloat16)])
+@pytest.mark.parametrize("ws", [0, (1 << 23) + 16])
+def test_head_rows_far_apart(anywhere, M, H, xs, dtype, ws):
+    """Rows more than 8 MiB apart, by their strides or their lengths: every call is one
+    that the C ABI takes, and together they are all the rows."""
+    from lps import _lib
+    V, n = 2, -(-H // 32)
+    w = lps.Mx4Tensor(_strided(V, 16 * n, max(ws, 16 * n)), torch.full((V, n), 127, dtype=torch.uint8), H)
+    if dtype == "mx4":
+        x = lps.Mx4Tensor(_strided(M, 16 * n, xs), torch.full((M, n), 127, dtype=torch.uint8), H)
+    else:
+        x = torch.zeros((M - 1) * xs + H, dtype=dtype).as_strided((M, H), (xs, 1))
+    out, stats = lps.lm_head(x, w, return_stats=True)
+    assert out.shape == (M, V) and stats.shape == (M, 1, 2)
+    at = 0
+    for _, args in anywhere:
+        a = _lib.LmHeadMx4Args.from_buffer_copy(args)
+        assert a.rows == 1 or (a.x_stride * (1 if dtype == "mx4" else 2) <= 1 << 23 and a.x_stride >= (16 * n if dtype == "mx4" else H))
+        assert a.x_stride % (16 if dtype == "mx4" else 8) == 0 or a.rows == 1
+        assert a.w_stride <= 1 << 23 and a.x % 16 == 0 and a.w % 16 == 0
+        assert a.out == out.data_ptr() + at * V * out.element_size() and a.stats == stats.data_ptr() + at * 8
+        at += a.rows
+    assert at == M
