@@ -371,7 +371,8 @@ int lps_softmax(const lps_softmax_args* args, void* stream);
  * to x / 2^s (ties to the even code, 6 above it, the sign kept for zeros); a
  * block with a value that is not finite becomes scale 255, codes 0.  Values
  * past a row's end count as zeros.
- * lps_mx4_dequantize: codes and scales to x (rounded to x's type).
+ * lps_mx4_dequantize: codes and scales to x (rounded to x's type; values past its
+ * range, which scale bytes 253 and 254 hold in every type, are infinities).
  * Code rows begin on 4-byte lines; everything else at any element. */
 typedef struct lps_mx4_args {
   void* x;                        /* [rows, hidden] in dtype */
@@ -389,10 +390,12 @@ int lps_mx4_quantize(const lps_mx4_args* args, void* stream);
 int lps_mx4_dequantize(const lps_mx4_args* args, void* stream);
 
 /* LM head over a 4-bit weight, lps_lm_head otherwise (logits, statistics):
- * x in bf16, fp16 or 4 bits.  Any hidden; the codes of w past a row's end count
- * as zeros, those of a 4-bit x must be (lps_mx4_quantize leaves them so).
+ * x in bf16, fp16 or 4 bits (to 16 bits a value of w past fp32's range is an
+ * infinity).  Any hidden; the codes of w past a row's end count as zeros, those
+ * of a 4-bit x must be (lps_mx4_quantize leaves them so).
  * Rows of x and w begin on 16-byte lines, rows of scales on 4-byte lines;
- * strides are at most 8 MiB, vocab 2^21, hidden 2^24. */
+ * strides are at most 8 MiB, vocab 2^21, hidden 2^24 (16-bit x of more than 2^22:
+ * a row a call, whose stride does not count). */
 typedef struct lps_lm_head_mx4_args {
   const void* x;                  /* [rows, hidden] in dtype; 4-bit codes */
   const void* x_scales;           /* 4-bit x: uint8 [rows, ceil(hidden / 32)] */

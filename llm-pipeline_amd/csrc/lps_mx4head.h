@@ -173,8 +173,10 @@ __device__ __forceinline__ u32x4 m4_frag(uint32_t codes, float s) {
   return r;
 }
 
-// Eight fp16 as two bf16 fragments whose sum they are: the top 8 bits of each
-// (cut off), and the rest (at most 3 bits, exact; 0 for infinities and NaN).
+// Eight fp16 as two bf16 fragments whose sum they are: the top 8 bits of each (cut
+// off) and the rest (at most 3 bits, exact).  Where nothing is left, infinities and
+// NaN among them, two halves: a weight past fp32's range is an infinity, and a zero
+// times it would be NaN.
 __device__ __forceinline__ void m4_split(u32x4 x, u32x4& hi, u32x4& lo) {
 #pragma unroll
   for (int i = 0; i < 4; i++) {
@@ -182,11 +184,11 @@ __device__ __forceinline__ void m4_split(u32x4 x, u32x4& hi, u32x4& lo) {
 #pragma unroll
     for (int e = 0; e < 2; e++) {
       const float f = f16_to_f32((x[i] >> (16 * e)) & 0xFFFFu);
-      h[e] = __float_as_uint(f) & 0xFFFF0000u;
-      const bool fine = (h[e] & 0x7F800000u) != 0x7F800000u;
-      // (a NaN whose set bits are all below the cut stays one)
-      if (!fine && f != f) h[e] |= 0x00400000u;
-      r[e] = fine ? __float_as_uint(__fsub_rn(f, __uint_as_float(h[e]))) : 0u;
+      const uint32_t top = __float_as_uint(f) & 0xFFFF0000u, half = __float_as_uint(__fmul_rn(0.5f, f)) & 0xFFFF0000u;
+      const float rest = __fsub_rn(f, __uint_as_float(top));
+      const bool some = (top & 0x7F800000u) != 0x7F800000u && rest != 0.0f;
+      h[e] = some ? top : half;
+      r[e] = some ? __float_as_uint(rest) : half;
     }
     hi[i] = (h[0] >> 16) | h[1];
     lo[i] = (r[0] >> 16) | (r[1] & 0xFFFF0000u);

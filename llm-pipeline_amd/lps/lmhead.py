@@ -33,7 +33,8 @@ def lm_head(hidden: Union[torch.Tensor, Mx4Tensor], weight: Union[torch.Tensor, 
 
     ``weight`` may be 4-bit (``mx4_quantize``): then ``H`` is any number,
     ``hidden`` bf16, fp16 or 4-bit itself, and ``out_dtype`` bfloat16 by default
-    for 4-bit ``hidden``.  The products are exact and summed in fp32.  A 16-bit
+    for 4-bit ``hidden``.  The products are exact and summed in fp32 (to a
+    16-bit ``hidden`` a weight past float32's range is an infinity).  A 16-bit
     ``hidden`` that asks for a derivative is refused."""
     if isinstance(weight, Mx4Tensor) or isinstance(hidden, Mx4Tensor):
         return _lm_head_mx4(hidden, weight, out_dtype, return_stats)

@@ -173,8 +173,9 @@ def mx4_quantize(x: torch.Tensor) -> Mx4Tensor:
 
 
 def mx4_dequantize(t: Mx4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """The values ``[..., H]`` of a 4-bit tensor, in ``dtype`` (every one is
-    exact in bfloat16 and float32)."""
+    """The values ``[..., H]`` of a 4-bit tensor, in ``dtype`` (every one that
+    ``mx4_quantize`` gives is exact in bfloat16 and float32; those past float32's
+    range, which scale bytes 253 and 254 can hold, are infinities)."""
     t.check("t")
     code = D.code_of(dtype)
     codes, scales = t.rows()

@@ -81,3 +81,40 @@ def gradient(ids, grad, vocab, scale, out, out_dtype):
     rel, least = HALF[out_dtype]
     bound = (count.unsqueeze(1) + 2) * 2.0 ** -24 * mag + want.abs() * (rel + 2.0 ** -23) * 1.01 + least
     return want, bound
+
+
+def extreme_scales(V, H, M, dtype):
+    """(codes, scales, x) of a head whose weights' scales are the largest and the
+    smallest, one value a row: products of one term each, no sum to round."""
+    nb = -(-H // 32)
+    codes = torch.zeros((V, 16 * nb), dtype=torch.uint8)
+    scales = torch.full((V, nb), 127, dtype=torch.uint8)
+    n = torch.arange(V)
+    at = (n * 37) % H                                      # the row's column
+    code = (1 + n % 7 + 8 * (n // 7 % 2)).to(torch.uint8)
+    codes[n, at // 2] = code << (4 * (at % 2)).to(torch.uint8)
+    scales[n, at // 32] = torch.tensor([254, 253, 252, 0, 1, 2, 60, 141, 103])[n % 9].to(torch.uint8)
+    # 8 bits, 11 bits, the largest, the smallest (fp16's), powers of two
+    v = torch.tensor([1.0, -1.25, 1.0 + 2.0 ** -7, 3.0 if dtype == torch.bfloat16 else 1.0 + 2.0 ** -10, 2.0 ** 15, -2.0 ** -24,
+                      2.0 ** -3])
+    x = v[(torch.arange(M)[:, None] + torch.arange(H)) % 7].to(dtype)
+    x[0, 37], x[M - 1, H - 1] = float("inf"), float("-inf")
+    return codes, scales, x
+
+
+def extreme_products(codes, scales, x):
+    """x times those weights as fp32: a weight past its range is an infinity."""
+    w = values(codes, scales, x.shape[1]).float().double()
+    n = torch.arange(w.shape[0])
+    at = (n * 37) % x.shape[1]
+    out = x.double()[:, at] * w[n, at]
+    # (an infinite state times one of the row's zeros)
+    infinite = torch.isinf(x.double())
+    return torch.where(infinite.sum(1, keepdim=True) > infinite[:, at].long(), float("nan"), out).float().double()
+
+
+def check_extreme(out, ref):
+    """Equal but for products under fp32's normal range, which matrix cores need not keep."""
+    out, fine = out.double().cpu(), torch.isfinite(ref)
+    assert torch.equal(out[~fine].nan_to_num(nan=0.125), ref[~fine].nan_to_num(nan=0.125))
+    assert bool(((out - ref)[fine].abs() <= torch.where(ref[fine].abs() < 2.0 ** -126, 2.0 ** -126, 0.0)).all())

@@ -227,3 +227,15 @@ def test_head_rows_far_apart(dev, M, H, xs, dtype):
     ref = torch.stack([x.double() @ R.values(codes[v:v + 1], scales[v:v + 1], H)[0] for v in range(V)], 1)
     assert torch.equal(out.double().cpu(), ref)
     assert torch.equal(stats[..., 0].double().cpu(), ref.amax(1, keepdim=True))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,H", [(3, 290), (70, 290), (20, 1024)])
+def test_head_weights_past_fp32(dev, dtype, M, H):
+    """The largest and the smallest scale bytes: values past fp32's range are
+    infinities to 16-bit states, as to the dequantiser."""
+    V = 517
+    c, s, x = R.extreme_scales(V, H, M, dtype)
+    t = lps.Mx4Tensor(c.to(dev), s.to(dev), H)
+    assert torch.equal(lps.mx4_dequantize(t, torch.float32).cpu(), R.values(c, s, H).float())
+    R.check_extreme(lps.lm_head(x.to(dev), t, out_dtype=torch.float32), R.extreme_products(c, s, x))

@@ -206,3 +206,22 @@ def test_head(run_table, tmp_path, monkeypatch, M, V, H, dtype, out_dtype):
         mx = blocks.max(dim=2).values
         assert torch.equal(st[..., 0], mx)
         torch.testing.assert_close(st[..., 1], torch.exp(blocks - mx.unsqueeze(-1)).sum(dim=2), rtol=2e-6, atol=0)
+
+
+@pytest.mark.parametrize("M", [3, 70])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_head_weights_past_fp32(run_table, tmp_path, monkeypatch, M, dtype):
+    """Scale bytes 253 and 254, which the quantiser never gives, hold values past
+    fp32's largest: infinities to 16-bit states, as to the dequantiser, whatever else
+    the row holds and however a state is taken apart."""
+    monkeypatch.setenv("LPS_EMU_CUS", "1")
+    V, H = 130, 290
+    c, s, x = R.extreme_scales(V, H, M, dtype)
+    nb, xs = s.shape[1], H + -H % 8
+    ss = nb + -nb % 4
+    pad = torch.cat([s, torch.full((V, ss - nb), 255, dtype=torch.uint8)], 1).reshape(-1)[:(V - 1) * ss + nb]
+    wide = torch.zeros((M, xs), dtype=dtype)
+    wide[:, :H] = x
+    out, _ = _take(_run(run_table, tmp_path, (4, DT[dtype], DT[torch.float32], M, V, H, xs, ss),
+                        wide.reshape(-1)[:(M - 1) * xs + H], c, pad), (torch.float32, M, V), (torch.float32, M, 2, 2))
+    R.check_extreme(out, R.extreme_products(c, s, x))
