@@ -239,3 +239,43 @@ def test_head_weights_past_fp32(dev, dtype, M, H):
     t = lps.Mx4Tensor(c.to(dev), s.to(dev), H)
     assert torch.equal(lps.mx4_dequantize(t, torch.float32).cpu(), R.values(c, s, H).float())
     R.check_extreme(lps.lm_head(x.to(dev), t, out_dtype=torch.float32), R.extreme_products(c, s, x))
+
+
+# (rows, vocab, states' type) such that each tile shape is taken on 256 CUs: a grid that
+# runs at once takes the smallest tiles, so the larger ones need many columns.
+SHAPES = ([(M, V, d) for d in (torch.bfloat16, torch.float16)
+           for M, V in ((7, 301), (16, 301), (31, 301), (64, 32897), (130, 22001))] +
+          [(30, 301, "mx4"), (64, 16601, "mx4"), (128, 16601, "mx4"), (300, 22001, "mx4")])
+# part of a block after whole stages; whole stages; a block and a part after more stages than the rings hold
+COLUMNS = {torch.float32: 1380, torch.bfloat16: 2048, torch.float16: 4139}
+
+
+@pytest.mark.parametrize("out_dtype", list(COLUMNS))
+@pytest.mark.parametrize("M,V,dtype", SHAPES)
+def test_every_tile_shape(dev, M, V, dtype, out_dtype):
+    """Each kernel at an odd vocabulary, against the products in fp64 on the GPU, with
+    block statistics; of fp16, rows whose scales it does not hold."""
+    H = COLUMNS[out_dtype]
+    g = torch.Generator(device=dev).manual_seed(M + V + H)
+    t = lps.mx4_quantize((torch.randn((V, H), generator=g, device=dev) * (2.0 / H ** 0.5)).bfloat16())
+    far = dtype == torch.float16
+    if far:                  # tiny, and where no sum of exponentials is compared huge
+        t.scales[::5, 3:9] -= 20
+        if out_dtype == torch.float32:
+            t.scales[1::5] += 25
+    x = torch.randn((M, H), generator=g, device=dev).to(torch.bfloat16 if dtype == "mx4" else dtype)
+    arg = lps.mx4_quantize(x) if dtype == "mx4" else x
+    out, stats = lps.lm_head(arg, t, out_dtype=out_dtype, return_stats=True)
+    again, again_stats = lps.lm_head(arg, t, out_dtype=out_dtype, return_stats=True)
+    assert torch.equal(out, again) and torch.equal(stats, again_stats)
+    xv = lps.mx4_dequantize(arg, torch.float32).double() if dtype == "mx4" else x.double()
+    w = lps.mx4_dequantize(t, torch.float32).double()
+    ref, mag = xv @ w.T, xv.abs() @ w.abs().T
+    half, least = R.HALF[out_dtype]
+    off = (out.double() - ref).abs() - (half * 1.01 * ref.abs() + H * 2.0 ** -24 * mag + least)
+    assert bool((off <= 0).all()), f"past the bound by {float(off.max())}"
+    if far and out_dtype == torch.float32:
+        blocks = torch.cat([out, torch.full((M, -V % 128), float("-inf"), device=dev)], 1).reshape(M, -1, 128)
+        assert torch.equal(stats[..., 0], blocks.amax(2))
+    else:
+        _check_stats(out, stats)

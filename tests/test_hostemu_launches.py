@@ -85,3 +85,19 @@ def test_gradients_of_huge_vocabularies(launches, n, vocab, hidden, dtype):
 def test_gradients_of_more_tiles_than_a_grid(launches):
     """Sizes past it are refused before any launch."""
     assert launches(GRADIENT, BF16, F32, 1 << 30, 1000, 16 * 2048 + 1) == (1, [])
+
+
+def test_gpu_cases_reach_every_tile_shape(launches):
+    """The kernels that some call can launch are those that the GPU tests' cases launch."""
+    import torch
+    from tests.test_gpu_mx4head import COLUMNS, SHAPES
+    code = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16, "mx4": MX4}
+
+    def kernel(M, V, dtype, out_dtype):
+        rc, made = launches(HEAD, dtype, out_dtype, M, V, COLUMNS[torch.float32])
+        assert fits(rc, made) and len(made) == 1
+        return made[0].kernel
+    tested = {kernel(M, V, code[d], code[o]) for M, V, d in SHAPES for o in COLUMNS}
+    reached = {kernel(M, V, d, o) for d in (BF16, F16, MX4) for o in (F32, BF16, F16)
+               for M in (1, 9, 17, 33, 65, 129, 257, 2000) for V in (1, 16601, 22001, 151936)}
+    assert reached == tested and len(tested) == len(SHAPES) * len(COLUMNS)
