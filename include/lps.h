@@ -357,7 +357,8 @@ int lps_softmax(const lps_softmax_args* args, void* stream);
 /* ------------------------------------------------------------------------
  * The vocabulary table: one [vocab, hidden] table at both ends of a decode
  * loop (the sampled token's row in, the LM head's products out), in 16 or 32
- * bits or as microscaled 4-bit floats.
+ * bits or as microscaled 4-bit floats.  A row has at most 2^24 values (16776960 in
+ * lps_embedding_grad).
  *
  * 4-bit form of a row: blocks of 32 values (the last may hold fewer), 16 bytes
  * of codes and one scale byte a block.  Scale byte b stands for 2^(b - 127),

@@ -4,7 +4,7 @@
 // call's result never depends on timing.
 //
 // Up to EG_SMALL positions grad_small_kernel, after grad_zero_kernel where there are
-// many zeros to write.  More, three launches:
+// many zeros to write; of none grad_zero_kernel alone.  More, three launches:
 // 1. grad_sort_kernel groups the positions by id.  Workgroup w of G takes the
 //    ids with id % G == w (neighbouring frequent ids land apart); it reads all
 //    ids, counts its own and those of the workgroups before it (its place in

@@ -12,14 +12,14 @@
 // terms is free, so a lane takes a whole block of w again (lanes l and l + 32
 // neighbouring ones) and spends it over four instructions, against the chunks of
 // x that belong to it: w is read from LDS in 16 bytes a lane, once, with one
-// scale a lane.  bf16 holds every value of w.  fp16 holds those of scales 2^-23 ..
+// scale a lane.  bf16 holds every value of w that fp32 does.  fp16 holds those of scales 2^-23 ..
 // 2^13; a stage in which a wave meets another scale takes x apart into two bf16
 // (11 bits as 8 and 3) and runs the bf16 instruction twice, which is exact too.
 //
 // What bounds it: up to ~32 rows w's pass over HBM (1 row of 4096 -> 151936: 58 us, 5.7
 // TB/s; a read reaches 7.0), from ~128 rows of 16 bits the matrix cores (2048 rows 2.15
 // ms, 1.19 PFLOP/s; the library's bf16 product takes 2.10) and from ~256 of 4 bits they
-// and the writing of the logits (2048 rows 764 us, 3.3 PFLOP/s).  Between them (64 rows
+// and the writing of the logits (2048 rows 768 us, 3.3 PFLOP/s).  Between them (64 rows
 // of 16 bits 101 us) stages of x and w wait for each other's latency: two workgroups of
 // 72 KB LDS on a CU are worth more than a deeper ring in one (64 x 128 tiles with 5
 // stages of w ahead 120 us; 64 x 256 tiles 111), and so are x held in registers with w
